@@ -236,9 +236,9 @@ def run_scan_train(s):
         last, first = cu[1:] - 1, cu[:-1]
         up = torch.cat([rho[1:], torch.zeros_like(rho[:1])])
         up[last] = 0
-        g = dy.float()
-        g[last] += s["dfinal"]
-        g = plain_scan(up.flip(0), g.flip(0)).flip(0)
+        g = dy.float().flip(0)  # a copy: the inputs stay as they are
+        g[dy.shape[0] - 1 - last] += s["dfinal"]
+        g = plain_scan(up.flip(0), g).flip(0)
         before = torch.cat([torch.zeros_like(h[:1]), h[:-1]])
         before[first] = s["initial"]
         drho = g * (before - x) if complement else g * before
