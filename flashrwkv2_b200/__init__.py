@@ -1,4 +1,5 @@
-"""B200-native (sm_100a) WKV7 time-mix recurrence behind FlashRWKV2's operator contract.
+"""B200-native (sm_100a) WKV7 time-mix recurrence behind FlashRWKV2's operator contract, with the operators that its
+users need beside it: the gated scan (elementwise recurrence) and token log probabilities behind the head.
 
 Backend selection mirrors rwkv-rs/FlashRWKV2 flashrwkv2/__init__.py:12-55: the private
 native module is chosen by compute capability and published as ``flashrwkv2_b200._C``.
@@ -46,6 +47,11 @@ def _load_native_backend():
 
 _C = _load_native_backend()
 
+from .head import TokenLogprobs, rl_infctx_head_token_logprobs  # noqa: E402
+from .tmix.gated_scan import (  # noqa: E402
+    infer_tmix_gated_scan_fp32io16_forward_varlen,
+    pretrain_tmix_gated_scan_fp32io16,
+)
 from .tmix.wkv7 import (  # noqa: E402
     infer_tmix_wkv7_fused_gate_fp32io16_forward_varlen,
     infer_tmix_wkv7_prefill_fp32io16_forward_varlen,
@@ -58,12 +64,16 @@ from .tmix.wkv7 import (  # noqa: E402
 )
 
 __all__ = [
+    "TokenLogprobs",
+    "infer_tmix_gated_scan_fp32io16_forward_varlen",
     "infer_tmix_wkv7_fused_gate_fp32io16_forward_varlen",
     "infer_tmix_wkv7_prefill_fp32io16_forward_varlen",
     "infer_tmix_wkv7_readout_fp32io16_forward_varlen",
     "infer_tmix_wkv7_recurrent_fp16_forward_varlen",
     "infer_tmix_wkv7_recurrent_fp32io16_forward_varlen",
     "prepare_tmix_wkv7_recurrent_metadata",
+    "pretrain_tmix_gated_scan_fp32io16",
     "pretrain_tmix_wkv7_recurrent_bf16",
+    "rl_infctx_head_token_logprobs",
     "rl_infctx_tmix_wkv7_chunk_fp32io16",
 ]

@@ -12,8 +12,9 @@ LIB_PATH = Path(__file__).resolve().parent / "lib" / "libfrwkv_sm100.so"
 
 IO_BF16, IO_FP16, IO_FP32 = 0, 1, 2
 DECAY_LOGITS, DECAY_RETENTION = 0, 1
+INPUT_UNIT, INPUT_COMPLEMENT = 0, 1
 PREFILL_AUTO, PREFILL_RECURRENT, PREFILL_CHUNK_TC = 0, 1, 2
-ABI_VERSION = 2
+ABI_VERSION = 3
 STATIC_POOL_SLOTS = 65536
 
 # every symbol include/frwkv_sm100.h declares
@@ -32,6 +33,12 @@ SYMBOLS = (
     "frwkv_sm100_wkv7_prefill_readout",
     "frwkv_sm100_wkv7_pretrain_forward",
     "frwkv_sm100_wkv7_pretrain_backward",
+    "frwkv_sm100_gated_scan_workspace_bytes",
+    "frwkv_sm100_gated_scan",
+    "frwkv_sm100_gated_scan_train_forward",
+    "frwkv_sm100_gated_scan_train_backward",
+    "frwkv_sm100_token_logprobs",
+    "frwkv_sm100_token_logprobs_backward",
 )
 
 _lib = None
@@ -87,6 +94,19 @@ def declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.frwkv_sm100_wkv7_pretrain_forward.argtypes = [vp] * 9 + [ci, ci, ci, vp]
     lib.frwkv_sm100_wkv7_pretrain_backward.restype = ci
     lib.frwkv_sm100_wkv7_pretrain_backward.argtypes = [vp] * 15 + [ci, ci, ci, vp]
+    ll = ctypes.c_longlong
+    lib.frwkv_sm100_gated_scan_workspace_bytes.restype = sz
+    lib.frwkv_sm100_gated_scan_workspace_bytes.argtypes = [ci, ci]
+    lib.frwkv_sm100_gated_scan.restype = ci
+    lib.frwkv_sm100_gated_scan.argtypes = [vp] * 5 + [ll, vp, ll, vp, vp] + [ci] * 7 + [vp, sz, vp]
+    lib.frwkv_sm100_gated_scan_train_forward.restype = ci
+    lib.frwkv_sm100_gated_scan_train_forward.argtypes = [vp] * 3 + [ll, vp, ll] + [vp] * 4 + [ci] * 6 + [vp, sz, vp]
+    lib.frwkv_sm100_gated_scan_train_backward.restype = ci
+    lib.frwkv_sm100_gated_scan_train_backward.argtypes = [vp] * 3 + [ll, vp, ll] + [vp] * 7 + [ci] * 6 + [vp, sz, vp]
+    lib.frwkv_sm100_token_logprobs.restype = ci
+    lib.frwkv_sm100_token_logprobs.argtypes = [vp] + [ll] * 4 + [vp, ci, ll] + [ci, ci, cf, ci] + [vp] * 6
+    lib.frwkv_sm100_token_logprobs_backward.restype = ci
+    lib.frwkv_sm100_token_logprobs_backward.argtypes = [vp] + [ll] * 4 + [vp, ci, ll] + [ci, ci, cf] + [vp] * 6
     return lib
 
 

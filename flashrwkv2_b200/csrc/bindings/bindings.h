@@ -9,3 +9,5 @@ void register_flashrwkv2_bindings(py::module_& module);
 void register_infer_tmix_wkv7_recurrent_fp32io16_bindings(py::module_& module);
 void register_rl_infctx_tmix_wkv7_chunk_forward_bindings(py::module_& module);
 void register_pretrain_tmix_wkv7_recurrent_bindings(py::module_& module);
+void register_tmix_gated_scan_bindings(py::module_& module);
+void register_rl_infctx_head_token_logprobs_bindings(py::module_& module);

@@ -1,0 +1,48 @@
+"""Gated scan: the elementwise sibling of the WKV7 recurrence, one fp32 number of state per (sequence, channel).
+
+    h_t = rho_t * h_{t-1} + i_t * x_t        y_t = h_t
+
+``decay_mode`` is WKV7's: "logits" (``rho = exp(-e^{-1/2} * sigmoid(logit + bias))``) or "retention" (``rho`` itself).
+``input_mode`` says what enters the state: "unit" (``i_t = 1``) or "complement" (``i_t = 1 - rho_t``, an exponential
+moving average with a data-dependent rate).  Tokens are bfloat16, float16 or float32; the state is float32.
+
+* :func:`infer_tmix_gated_scan_fp32io16_forward_varlen` serves packed sequences (decode steps and prompts of any length)
+  in place on a state pool, with the metadata ticket of the WKV7 operators: one ticket serves both in a step.
+* :func:`pretrain_tmix_gated_scan_fp32io16` is differentiable, over dense or packed rows, with an initial state that
+  takes a gradient and a final state that gives one.
+
+Errors: ``TypeError`` for wrong types, ``ValueError`` for wrong shapes, layouts and values, before any launch.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from ..wkv7 import _extension, prepare_tmix_wkv7_recurrent_metadata
+from .pretrain import pretrain_tmix_gated_scan_fp32io16
+
+
+def infer_tmix_gated_scan_fp32io16_forward_varlen(
+        x: torch.Tensor, decay_logits: torch.Tensor, *, state_pool: torch.Tensor, cu_seqlens: torch.Tensor,
+        state_indices: torch.Tensor, decay_bias: torch.Tensor | None = None, max_seqlen: int | None = None,
+        validated_metadata: object | None = None, decay_mode: str = "logits",
+        input_mode: str = "unit") -> torch.Tensor:
+    """Packed gated scan, in place on ``state_pool`` at ``state_indices``; returns y.
+
+    ``x`` and ``decay_logits`` are ``[total_tokens, C]`` (rows may lie apart, as in a slice of a wider projection),
+    ``state_pool`` float32 ``[slots, C]``, ``decay_bias`` ``[C]`` (logits mode only).  Metadata, tickets, CUDA-graph use and
+    the fail-closed rules are those of the WKV7 operators: without ``validated_metadata`` the metadata is checked on the
+    host (one sync); with a capacity ticket nothing synchronises, rows behind the last active sequence are left as they
+    were allocated, and invalid metadata fills y with NaN and leaves the pool untouched.  A call needs its scratch to
+    itself until it has finished, which torch's allocator sees to; captured graphs own theirs."""
+    native = _extension()
+    if validated_metadata is None and isinstance(x, torch.Tensor) and isinstance(state_pool, torch.Tensor) and x.is_cuda:
+        validated_metadata = prepare_tmix_wkv7_recurrent_metadata(
+            cu_seqlens, state_indices, total_tokens=x.shape[0], state_pool_size=state_pool.shape[0],
+            max_seqlen=max_seqlen)
+    return native.tmix_gated_scan_fp32(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias,
+                                       validated_metadata, -1 if max_seqlen is None else max_seqlen, decay_mode,
+                                       input_mode)
+
+
+__all__ = ["infer_tmix_gated_scan_fp32io16_forward_varlen", "pretrain_tmix_gated_scan_fp32io16"]

@@ -27,7 +27,8 @@
 extern "C" {
 #endif
 
-#define FRWKV_SM100_ABI_VERSION 2 /* 2: fp16-state, fused-gate, readout and training entries added; the entries of 1 unchanged */
+#define FRWKV_SM100_ABI_VERSION 3 /* 2: fp16-state, fused-gate, readout and training entries added; 3: gated scan and token
+                                     log probabilities added; the entries of 1 and 2 unchanged */
 
 /* token dtype of r,w,k,v,a,b,y */
 enum { FRWKV_IO_BF16 = 0, FRWKV_IO_FP16 = 1, FRWKV_IO_FP32 = 2 };
@@ -40,6 +41,8 @@ enum { FRWKV_IO_BF16 = 0, FRWKV_IO_FP16 = 1, FRWKV_IO_FP32 = 2 };
  * entry's error_flag instead of passing inf/NaN on silently.  The recurrent entry and FRWKV_PREFILL_RECURRENT take
  * any rho in [0, 1]. */
 enum { FRWKV_DECAY_LOGITS = 0, FRWKV_DECAY_RETENTION = 1 };
+/* what a gated scan feeds its state with: x_t itself, or (1 - rho_t) * x_t (an exponential moving average) */
+enum { FRWKV_INPUT_UNIT = 0, FRWKV_INPUT_COMPLEMENT = 1 };
 /* metadata error bits written to status[0]; same values as
  * csrc/validation/recurrent_metadata.cu:15-22 */
 enum {
@@ -236,6 +239,68 @@ int frwkv_sm100_wkv7_pretrain_backward(const void* r, const void* w, const void*
                                        const void* b, const void* dy, const float* boundary,
                                        const float* state_dot_a, void* dr, void* dw, void* dk, void* dv, void* da,
                                        void* db, int batch, int tokens, int heads, void* stream);
+
+/* Gated scan: the elementwise sibling of the WKV7 recurrence, one fp32 number of state per (sequence, channel),
+ *   h_t = rho_t * h_{t-1} + i_t * x_t,   y_t = h_t,   i_t = 1 or 1 - rho_t (FRWKV_INPUT_*),
+ * with rho from decay logits (+ bias) or the retention itself (FRWKV_DECAY_*).  No counterpart in the reference.
+ *   x, decay   : [total_tokens, channels] in the token dtype (bf16, fp16 or fp32), unit channel stride, rows
+ *                x_row_stride / decay_row_stride elements apart;  decay_bias : [channels] in the token dtype or NULL;
+ *   state_pool : fp32 [pool_slots, channels], updated in place at slots[seq] only;
+ *   y          : [total_tokens, channels], contiguous, token dtype;
+ *   cu_seqlens, slots, status, max_seqlen : as in frwkv_sm100_wkv7_recurrent, with the same fail-closed rules
+ *                (invalid metadata: y NaN-filled, pool untouched; rows behind the last active sequence untouched);
+ *   workspace  : device scratch of frwkv_sm100_gated_scan_workspace_bytes(total_tokens, channels) bytes, 16-byte
+ *                aligned, for this call alone until it has finished (two calls that may overlap need two).
+ * Any number of channels; channels and strides that are multiples of 8 (16-byte rows) run fastest. */
+size_t frwkv_sm100_gated_scan_workspace_bytes(int total_tokens, int channels);
+int frwkv_sm100_gated_scan(
+    const int32_t* cu_seqlens, const int32_t* slots, const int32_t* status, float* state_pool, const void* x,
+    long long x_row_stride, const void* decay, long long decay_row_stride, const void* decay_bias, void* y, int n_seq,
+    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* workspace,
+    size_t workspace_bytes, void* stream);
+
+/* The gated scan as a training operator.  Rows are n_seq sequences of total_tokens / n_seq tokens each (cu_seqlens
+ * NULL), or packed by cu_seqlens [n_seq+1], whose status word then rules as above (invalid: outputs NaN-filled).
+ *   initial  : fp32 [n_seq, channels] or NULL (zeros);   final_state : fp32 [n_seq, channels];
+ *   boundary : fp32 [ceil(total_tokens / FRWKV_GATED_SCAN_TILE), channels], saved for the backward pass: the state
+ *              before the first token of every tile of rows;
+ *   dy, dx, ddecay : contiguous, token dtype;  dfinal (NULL: zeros), dinitial (NULL: not wanted) : fp32. */
+#define FRWKV_GATED_SCAN_TILE 64
+int frwkv_sm100_gated_scan_train_forward(
+    const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
+    long long decay_row_stride, const float* initial, void* y, float* final_state, float* boundary, int n_seq,
+    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, void* workspace,
+    size_t workspace_bytes, void* stream);
+int frwkv_sm100_gated_scan_train_backward(
+    const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
+    long long decay_row_stride, const float* initial, const float* boundary, const void* dy, const float* dfinal,
+    void* dx, void* ddecay, float* dinitial, int n_seq, int total_tokens, int channels, int io_dtype, int decay_mode,
+    int input_mode, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens under rows of vocabulary logits, with the entropy of each row and its most
+ * probable tokens; forward and gradient.  No counterpart in the reference.  z = logits / temperature,
+ *   logprob = z[id] - logsumexp(z),   entropy = logsumexp(z) - sum_j p_j z_j,   p = softmax(z),
+ *   dlogits_j = (dlogprob * ([j = id] - p_j) - dentropy * p_j * (log p_j + entropy)) / temperature.
+ *   logits   : outer * inner rows of `vocab` elements (bf16, fp16 or fp32), unit stride inside a row, row (o, i) at
+ *              o * stride_outer + i * stride_inner elements; every array below has one entry per row in that order;
+ *   ids      : int64 (ids_are_int64 nonzero) or int32; an id equal to ignore_index marks a row that
+ *              is left out (logprob, entropy and gradient 0, top ids -1 and top logprobs -inf, logits not read); any
+ *              other id outside [0, vocab) gives logprob and gradient NaN;
+ *   stats    : fp32 [rows, 2], the row's largest logit and log sum exp(z - max z): saved for the backward pass;
+ *   top_ids  : int64 [rows, top_k], top_logprobs : fp32 [rows, top_k]; top_k in 0..FRWKV_TOP_K_MAX and <= vocab;
+ *              descending, equal logits in the order of their ids (NaN counts as the largest);
+ * A row of -inf alone has logprob and top logprobs -inf, entropy 0 and gradient 0; a NaN or +inf in a row makes its
+ * logprobs, entropy and gradient NaN.  dlogprobs / dentropy : fp32 or NULL (zeros);  dlogits : contiguous [rows, vocab]. */
+#define FRWKV_TOP_K_MAX 32
+int frwkv_sm100_token_logprobs(
+    const void* logits, long long outer, long long inner, long long stride_outer, long long stride_inner,
+    const void* ids, int ids_are_int64, long long ignore_index, int vocab, int io_dtype, float temperature, int top_k,
+    float* logprobs, float* entropy, float* stats, int64_t* top_ids, float* top_logprobs, void* stream);
+int frwkv_sm100_token_logprobs_backward(
+    const void* logits, long long outer, long long inner, long long stride_outer, long long stride_inner,
+    const void* ids, int ids_are_int64, long long ignore_index, int vocab, int io_dtype, float temperature,
+    const float* stats, const float* entropy, const float* dlogprobs, const float* dentropy, void* dlogits,
+    void* stream);
 
 #ifdef __cplusplus
 }
