@@ -28,6 +28,7 @@ constexpr int kClusterCtas = 512;      // no more CTAs than this by splitting ro
 constexpr int kClusterBytes = 16384;   // and no part of a row smaller than this (one batch of a CTA)
 // exp2 of anything below is 0 in fp32; keeps 0 * -inf out of W and of the gradient
 constexpr float kLowest = -160.0f;
+constexpr float kSlack = 4.0f;  // how far, in powers of two, a logit may lie above the reference of a thread's sums
 
 struct Rows {
   const void* logits;
@@ -132,28 +133,39 @@ template <typename io_t> __device__ __forceinline__ float largest(const Pack<io_
   }
 }
 
-// Running maximum of the raw logits and the sums relative to it (two lanes each, for packed fp32 arithmetic).
+// A thread's largest logit, and its sums relative to a reference logit m that is not far below it (two lanes each, for
+// packed fp32 arithmetic).  The reference moves only when a batch exceeds it by more than 2^kSlack in the exponential: with
+// the maximum itself as reference some lane of a warp would move it in almost every batch.  An exponent of kSlack costs
+// no more precision than one of -kSlack.
 struct Sums {
-  float m;
+  float top, m;
   float2 s, w;
+  float next;  // the largest logit outside the batch that holds `top`
+  int top_batch;
 
   __device__ __forceinline__ void clear() {
-    m = -INFINITY;
+    top = next = m = -INFINITY;
+    top_batch = 0;
     s = w = make_float2(0.f, 0.f);
   }
-  // moves the sums to a larger maximum: e_j becomes e_j f and z_j becomes z_j + c, f = 2^c
-  __device__ __forceinline__ void rise(float top, float k) {
+  // moves the sums to a larger reference: e_j becomes e_j f and z_j becomes z_j + c, f = 2^c
+  __device__ __forceinline__ void rise(float to, float k) {
     if (m != -INFINITY) {
-      const float c = fmaxf((m - top) * k, kLowest), f = exp2_fast(c);
+      const float c = fmaxf((m - to) * k, kLowest), f = exp2_fast(c);
       w = make_float2(f * fmaf(c, s.x, w.x), f * fmaf(c, s.y, w.y));
       s = make_float2(f * s.x, f * s.y);
     }
-    m = top;
+    m = to;
   }
-  template <typename io_t> __device__ __forceinline__ void add(const Pack<io_t> (&v)[kBatch], float k) {
-    const float top = largest(v);
-    if (top == -INFINITY) return;
-    if (top > m) rise(top, k);
+  template <typename io_t, bool TOP> __device__ __forceinline__ void add(const Pack<io_t> (&v)[kBatch], int batch, float k) {
+    const float most = largest(v);
+    if (most == -INFINITY) return;
+    if ((most - m) * k > kSlack) rise(most, k);
+    if constexpr (TOP) {
+      next = fmaxf(next, fminf(top, most));
+      top_batch = most > top ? batch : top_batch;
+    }
+    top = fmaxf(top, most);
     const float2 minus_m = make_float2(-m, -m), k2 = make_float2(k, k);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
@@ -169,28 +181,32 @@ struct Sums {
   }
   __device__ __forceinline__ void add(float x, float k) {
     if (x == -INFINITY) return;
-    if (x > m) rise(x, k);
+    if ((x - m) * k > kSlack) rise(x, k);
+    top = fmaxf(top, x);
     const float z = max_keep_nan((x - m) * k, kLowest), e = exp2_fast(z);
     s.x += e;
     w.x = fmaf(e, z, w.x);
   }
 };
 
+// Largest logit, and sums relative to it (relative to m before they are joined).
 struct Total {
   float m, s, w;
 };
 
-// Sums of two parts relative to the larger maximum.  A part without a finite maximum holds nothing, or NaN.
-__device__ __forceinline__ Total join(const Total& a, const Total& b, float k) {
-  Total t{fmaxf(a.m, b.m), 0.f, 0.f};
+// Joins the totals of a warp's lanes; every lane gets the result.  All sums are moved to the common maximum of `top` and
+// added in a fixed tree.  A part without a reference holds nothing, or NaN.
+__device__ __forceinline__ Total join_lanes(float top, Total part, float k) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const Total& p = i == 0 ? a : b;
-    const float c = p.m == -INFINITY ? 0.f : fmaxf((p.m - t.m) * k, kLowest), f = exp2_fast(c);
-    t.w += f * fmaf(c, p.s, p.w);
-    t.s += f * p.s;
+  for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+  const float c = part.m == -INFINITY ? 0.f : fmaxf((part.m - top) * k, kLowest), f = exp2_fast(c);
+  float s = f * part.s, w = f * fmaf(c, part.s, part.w);
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, d);
+    w += __shfl_xor_sync(0xffffffffu, w, d);
   }
-  return t;
+  return Total{top, s, w};
 }
 
 // A CTA's part of a row: packs [first, last) behind `lead` single logits; the CTA that owns the singles takes those
@@ -208,29 +224,30 @@ template <typename io_t> struct Part {
 };
 
 struct TopScratch {
-  unsigned long long above[kAbove + kEqual];  // keys above the bar, and if they fit those equal to it behind them
-  unsigned long long equal[kEqual];
+  // keys above the bar, and from kAbove on those equal to it; the joined lists of a cluster
+  unsigned long long found[kAbove + kEqual];
   unsigned long long list[FRWKV_TOP_K_MAX];  // the answer: descending keys, 0 where there are fewer
   unsigned long long warp_best[kWarps];
   unsigned bars[kWarps];
-  int hot[kThreads], warp_count[kWarps];
-  int hot_count, above_count, equal_count;
+  int hot[kThreads], wide[kThreads], warp_count[kWarps];
+  int hot_count, wide_count, above_count, equal_count;
 };
 
 // Writes the CTA's top_k keys into t.list.
 //
-// While the sums were taken every thread kept its largest logit.  Each warp offers its ceil(top_k / 8)-th largest of these
-// 32; the smallest offer is a bar that at least top_k logits reach, and few more do (about 30 of 65536 for top_k 20).
-// Only the packs of threads whose largest logit reaches the bar are read again (from L2: 26 KB of a row of 128 KB), what
-// reaches it is collected and ranked by counting.  Logits equal to the bar count only as far as those above do not suffice;
-// where they are too many to collect (masked rows: -inf), the lowest ids among them are found in order.
-// Rows with NaN, and with more logits above the bar than there is room for, take top_k passes.
+// While the sums were taken every thread kept its largest logit, the batch of loads that held it and the largest one
+// outside that batch.  Each warp offers its ceil(top_k / 8)-th largest of these 32 maxima; the smallest offer is a bar that
+// at least top_k logits reach, and few more do (about 35 of 65536 for top_k 20).  Only the batches of the threads that
+// reach the bar are read again (a tenth of the row, from L2), all of a thread's batches where its second one may
+// reach it too; what reaches it is collected and ranked by counting.  Logits equal to the bar count only as far as those
+// above do not suffice; where they are too many to collect (masked rows: -inf), the lowest ids among them are found in
+// order.  Rows with NaN, and with more logits above the bar than there is room for, take top_k passes.
 template <typename io_t>
-__device__ void select_top(const Part<io_t>& part, float thread_max, bool has_nan, int top_k, TopScratch& t) {
+__device__ void select_top(const Part<io_t>& part, const Sums& sums, bool has_nan, int top_k, TopScratch& t) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < FRWKV_TOP_K_MAX) t.list[tid] = 0;
-  if (tid == 0) t.hot_count = t.above_count = t.equal_count = 0;
-  unsigned mine = order_of(thread_max), offer = 0;
+  if (tid == 0) t.hot_count = t.wide_count = t.above_count = t.equal_count = 0;
+  unsigned mine = order_of(sums.top), offer = 0;
   for (int r = 0; r < (top_k + kWarps - 1) / kWarps; ++r) {
     offer = __reduce_max_sync(0xffffffffu, mine);
     const unsigned who = __ballot_sync(0xffffffffu, mine == offer);
@@ -242,33 +259,46 @@ __device__ void select_top(const Part<io_t>& part, float thread_max, bool has_na
 #pragma unroll
   for (int w = 1; w < kWarps; ++w) bar_order = min(bar_order, t.bars[w]);
   const float bar = value_of(bar_order);
-  const auto offer_logit = [&](float x, int id) {
+  const auto consider_logit = [&](float x, int id) {
     if (x > bar) {
       const int at = atomicAdd(&t.above_count, 1);
-      if (at < kAbove) t.above[at] = rank_key(x, id);
+      if (at < kAbove) t.found[at] = rank_key(x, id);
     } else if (x == bar) {
       const int at = atomicAdd(&t.equal_count, 1);
-      if (at < kEqual) t.equal[at] = rank_key(x, id);
+      if (at < kEqual) t.found[kAbove + at] = rank_key(x, id);
     }
   };
-  const int count = part.last - part.first;
+  if (!any_nan && sums.top >= bar) {
+    t.hot[atomicAdd(&t.hot_count, 1)] = tid | sums.top_batch << 8;
+    if (sums.next >= bar) t.wide[atomicAdd(&t.wide_count, 1)] = tid | sums.top_batch << 8;
+  }
+  __syncthreads();
   if (!any_nan) {
-    if (thread_max >= bar) {
-      t.hot[atomicAdd(&t.hot_count, 1)] = tid;
-      for (int i = tid; i < part.single_count(); i += kThreads) offer_logit(to_f32(part.row[part.single(i)]), part.single(i));
-    }
-    __syncthreads();
-    const int rounds = (count + kThreads - 1) / kThreads, hot = t.hot_count;
-    for (int i = tid; i < hot * rounds; i += kThreads) {
-      const int pack = part.first + t.hot[i % hot] + i / hot * kThreads;
+    for (int i = tid; i < part.single_count(); i += kThreads) consider_logit(to_f32(part.row[part.single(i)]), part.single(i));
+    const int batches = (part.last - part.first + kBatch * kThreads - 1) / (kBatch * kThreads);
+    const int narrow = t.hot_count * kBatch, all = narrow + t.wide_count * batches * kBatch;
+    for (int i = tid; i < all; i += kThreads) {
+      int entry, batch;
+      if (i < narrow) {
+        entry = t.hot[i / kBatch];
+        batch = entry >> 8;
+      } else {
+        const int j = (i - narrow) / kBatch;
+        entry = t.wide[j / batches];
+        batch = j % batches;
+        if (batch == entry >> 8) continue;  // among the narrow ones
+      }
+      const int pack = part.first + (batch * kBatch + i % kBatch) * kThreads + (entry & 0xff);
       if (pack >= part.last) continue;
       Pack<io_t> v;
       v.load(part.row + part.pack_id(pack));
 #pragma unroll
       for (int j = 0; j < Pack<io_t>::kCount / 2; ++j) {
         const float2 x = v.pair(j);
-        offer_logit(x.x, part.pack_id(pack) + 2 * j);
-        offer_logit(x.y, part.pack_id(pack) + 2 * j + 1);
+        if (fmaxf(x.x, x.y) >= bar) {
+          consider_logit(x.x, part.pack_id(pack) + 2 * j);
+          consider_logit(x.y, part.pack_id(pack) + 2 * j + 1);
+        }
       }
     }
   }
@@ -310,12 +340,11 @@ __device__ void select_top(const Part<io_t>& part, float thread_max, bool has_na
   }
   const bool collected = equal <= kEqual;
   const int total = above + (collected ? equal : 0);
-  if (collected && tid < equal) t.above[above + tid] = t.equal[tid];
-  __syncthreads();
+  const auto found = [&](int i) { return t.found[i < above ? i : kAbove + i - above]; };
   for (int i = tid; i < total; i += kThreads) {
-    const unsigned long long key = t.above[i];
+    const unsigned long long key = found(i);
     int rank = 0;
-    for (int j = 0; j < total; ++j) rank += t.above[j] > key;
+    for (int j = 0; j < total; ++j) rank += found(j) > key;
     if (rank < top_k) t.list[rank] = key;
   }
   if (!collected) {
@@ -377,7 +406,7 @@ __device__ void select_top(const Part<io_t>& part, float thread_max, bool has_na
 // One row per CTA, or per cluster of CTAs that take equal parts of it (few rows: a row alone cannot fill the GPU).
 // Per thread: kBatch 16-byte loads in flight; the sums are rescaled only when a batch raises the running maximum.
 template <typename io_t, bool TOP>
-__global__ void __launch_bounds__(kThreads, 5)
+__global__ void __launch_bounds__(kThreads, 6)
 token_logprobs_kernel(const Rows p, int top_k, float* __restrict__ logprobs, float* __restrict__ entropy,
                       float* __restrict__ stats, int64_t* __restrict__ top_ids, float* __restrict__ top_logprobs) {
   __shared__ Total warp_total[kWarps];
@@ -416,6 +445,7 @@ token_logprobs_kernel(const Rows p, int top_k, float* __restrict__ logprobs, flo
   const float k = p.inv_temperature * kLog2e;
   Sums sums;
   sums.clear();
+  int batch = 0;
   for (int pack = part.first + tid; pack < part.last; pack += kBatch * kThreads) {
     Pack<io_t> v[kBatch];
 #pragma unroll
@@ -423,46 +453,48 @@ token_logprobs_kernel(const Rows p, int top_k, float* __restrict__ logprobs, flo
       if (pack + b * kThreads < part.last) v[b].load(part.row + part.pack_id(pack + b * kThreads));
       else v[b].fill_lowest();
     }
-    sums.add(v, k);
+    sums.template add<io_t, TOP>(v, batch++, k);
   }
   for (int i = tid; i < part.single_count(); i += kThreads) sums.add(to_f32(part.row[part.single(i)]), k);
 
   // thread, warp, CTA, cluster: always in the same order
-  Total mine{sums.m, sums.s.x + sums.s.y, sums.w.x + sums.w.y};
-  const bool has_nan = mine.s != mine.s;
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    const Total other{__shfl_xor_sync(0xffffffffu, mine.m, m), __shfl_xor_sync(0xffffffffu, mine.s, m),
-                      __shfl_xor_sync(0xffffffffu, mine.w, m)};
-    mine = (tid & m) == 0 ? join(mine, other, k) : join(other, mine, k);
-  }
-  if ((tid & 31) == 0) warp_total[tid >> 5] = mine;
-  if constexpr (TOP) select_top(part, sums.m, has_nan, top_k, top_scratch[0]);
+  const Total mine{sums.m, sums.s.x + sums.s.y, sums.w.x + sums.w.y};
+  const Total warp_sum = join_lanes(sums.top, mine, k);
+  if ((tid & 31) == 0) warp_total[tid >> 5] = warp_sum;
+  if constexpr (TOP) select_top(part, sums, mine.s != mine.s, top_k, top_scratch[0]);
   else __syncthreads();
-  Total all = warp_total[0];
-  for (int w = 1; w < kWarps; ++w) all = join(all, warp_total[w], k);
+  if (parts == 1 && tid >= 32) return;
+  const Total nothing{-INFINITY, 0.f, 0.f};
+  Total all = nothing;
+  if (tid < 32) {
+    all = tid < kWarps ? warp_total[tid] : nothing;
+    all = join_lanes(all.m, all, k);
+  }
   if (parts > 1) {
     if (tid == 0) cta_total = all;
     cluster.sync();
     if (rank == 0) {
-      for (int r = 1; r < parts; ++r) all = join(all, *cluster.map_shared_rank(&cta_total, r), k);
+      if (tid < 32) {
+        all = tid < parts ? *cluster.map_shared_rank(&cta_total, tid) : nothing;
+        all = join_lanes(all.m, all, k);
+      }
       if constexpr (TOP) {
-        // the parts' lists, joined by counting; a list is sorted, so entry i of one is above those behind it
+        // the parts' lists, joined by counting
         const int n = parts * top_k;
         for (int i = tid; i < n; i += kThreads)
-          top_scratch[0].above[i] = cluster.map_shared_rank(top_scratch[0].list, i / top_k)[i % top_k];
+          top_scratch[0].found[i] = cluster.map_shared_rank(top_scratch[0].list, i / top_k)[i % top_k];
         __syncthreads();
         for (int i = tid; i < n; i += kThreads) {
-          const unsigned long long key = top_scratch[0].above[i];
+          const unsigned long long key = top_scratch[0].found[i];
           int place = 0;
-          for (int j = 0; j < n; ++j) place += top_scratch[0].above[j] > key;
+          for (int j = 0; j < n; ++j) place += top_scratch[0].found[j] > key;
           if (key != 0 && place < top_k) top_scratch[0].list[place] = key;
         }
         __syncthreads();
       }
     }
     cluster.sync();  // rank 0 has read the others' shared memory
-    if (rank != 0) return;
+    if (rank != 0 || tid >= 32) return;
   }
   // a row of -inf alone has no maximum and no sum; NaN shows in the sum
   const bool empty = all.m == -INFINITY && all.s == 0.f;
