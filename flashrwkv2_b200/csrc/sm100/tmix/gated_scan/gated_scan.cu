@@ -1,17 +1,23 @@
 // Gated scan: in-place serving operator and training forward / backward (see gated_scan.cuh for the arithmetic).
 //
-// Rows are cut into tiles of kWarps * S consecutive tokens by 32 * V channels, without regard to sequences: a start inside
-// a tile cuts the recurrence there.  A lane owns V channels, a warp S tokens, whose gates and inputs stay in registers
-// from the only time they are read: one sweep gives the warp's affine map, the CTA joins the maps of its warps, the chain
-// (gated_scan.cuh) gives the state before the tile, a second sweep over the registers writes the rows.  So the tokens are
-// read once and the outputs written once, time is split over the whole GPU even for one sequence, and a batch of ragged
-// sequences is as regular as a dense one.
+// Rows are cut into tiles of 64 consecutive tokens by 256 bytes of channels, without regard to sequences: a start inside a
+// tile cuts the recurrence there.  A warp owns 8 tokens, a lane 8 bytes of channels.  The tokens come through shared
+// memory (cp.async, the next tile's while this one is worked on); a first sweep computes the gates into registers and
+// gives the warp's affine map, the CTA joins the maps of its warps, the chain (gated_scan.cuh) gives the state before the
+// tile, a second sweep writes the rows.  So the tokens are read once and the outputs written once, time is split over the
+// whole GPU even for one sequence, and a batch of ragged sequences is as regular as a dense one.
 #include "gated_scan.cuh"
 
 namespace frwkv {
 namespace {
 
 constexpr int kTile = FRWKV_GATED_SCAN_TILE;
+constexpr int S = 8, kWarps = 8, kThreads = kWarps * 32;
+#ifndef FC
+#define FC 3
+#endif
+constexpr int kForwardCtas = FC, kBackwardCtas = 2;  // per SM: 64 KB of staging each, 96 KB backward
+static_assert(S * kWarps == kTile, "the forward pass saves one state for each tile of the backward pass");
 
 // NaN in every row that the call would write (fail-closed), by the whole grid.
 template <typename io_t>
@@ -24,23 +30,37 @@ __device__ void fill_rows_nan(const GatedScanParams& p, io_t* rows, io_t* more_r
     fill_output_nan<float>(states, nullptr, static_cast<long long>(n_states) * p.channels, self, threads);
 }
 
+// Persistent CTAs take tiles in order and learn their next one a tile ahead; with one tile of rows there is no chain
+// and no counter.
+__device__ __forceinline__ int take_ticket(const ChainSpace& chain) { return atomicAdd(chain.ticket, 1) + 1; }
+
+// A CTA's tiles: time tile, channel block.  Persistent CTAs take tiles in order and learn their next one a tile ahead.
+struct Tile {
+  int time, block;  // time < 0: none left
+};
+
+// Which tile a ticket stands for; `tiles` of them are in use.
+__device__ __forceinline__ Tile tile_of(int ticket, int tiles, int blocks) {
+  if (ticket >= tiles) return Tile{-1, 0};
+  const int time = ticket / blocks;
+  return Tile{time, ticket - time * blocks};
+}
+
+__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" : : : "memory"); }
+template <int LEFT> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" : : "n"(LEFT) : "memory"); }
+
 // ---- forward
 
-template <typename io_t, int V, int S, int kWarps, bool LOGITS, bool COMPLEMENT>
-__global__ void __launch_bounds__(kWarps * 32, 1024 / (kWarps * 32))
-gated_scan_forward_kernel(const GatedScanParams p, const ChainSpace chain) {
+template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT>
+__global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_kernel(const GatedScanParams p, const ChainSpace chain) {
+  constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
-  using F = typename L::type;
-  using D = Decay<LOGITS, V>;
-  using W = Word<io_t, V>;
-  struct Piece {  // a warp's affine map
-    F a, b;
-  };
-  constexpr int kRows = kWarps * S;
-  __shared__ Piece pieces[kWarps][32];
+  using D = Decay<LOGITS, COMPLEMENT, V>;
+  using A = Access<io_t, GRANULE>;
+  extern __shared__ uint2 staged[];  // [2 tiles][warp][x or decay][S][lane]
+  __shared__ Map<V> pieces[kWarps][32];
   __shared__ unsigned cut[kWarps];
-  __shared__ F carry[32];
-  __shared__ int next_ticket[2];
+  __shared__ Tile coming[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, p.boundary != nullptr ? p.final_state : nullptr, p.n_seq);
@@ -48,116 +68,123 @@ gated_scan_forward_kernel(const GatedScanParams p, const ChainSpace chain) {
   }
   const int active = p.status != nullptr ? p.status[1] : p.total;
   const int n_seq = p.status != nullptr ? p.status[2] : p.n_seq;
-  const int tiles = (active + kRows - 1) / kRows * chain.blocks;  // of the rows in use
-  int round = 0, ticket = blockIdx.x;
-  if (chain.tiles > 1) {
-    if (threadIdx.x == 0) next_ticket[0] = atomicAdd(chain.ticket, 1);
-    __syncthreads();
-    ticket = next_ticket[0];
-  }
-  typename W::type raw_x[S], raw_d[S];
-  const auto fetch = [&](int t) {
-    if (t >= tiles) return;
-    const int row = t / chain.blocks * kRows + warp * S, channel = (t % chain.blocks * 32 + lane) * V;
-    const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
-    const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
+  const int tiles = (active + kTile - 1) / kTile * chain.blocks;  // of the rows in use
+  const bool chained = chain.tiles > 1;
+  if (threadIdx.x == 0) coming[0] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : blockIdx.x, tiles, chain.blocks);
+  __syncthreads();
+  Tile tile = coming[0];
+  const auto fetch = [&](const Tile& t, int buffer) {
+    if (t.time >= 0) {
+      const int row = t.time * kTile + warp * S, channel = (t.block * 32 + lane) * V;
+      const int count = min(V, p.channels - channel), rows = min(S, active - row);
+      const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
+      const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
+      uint2* to = staged + (buffer * kWarps + warp) * 2 * S * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const bool in = row + i < active && channel < p.channels;
-      raw_x[i] = in ? W::load(x + i * p.x_stride) : W::zero();
-      raw_d[i] = in ? W::load(d + i * p.decay_stride) : W::zero();
+      for (int i = 0; i < S; ++i) {
+        const int n = i < rows ? count : 0;
+        A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
+        A::stage(to + (S + i) * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
+      }
     }
+    copies_begun();
   };
-  fetch(ticket);
-  for (; ticket < tiles; ++round) {
-    const int time = ticket / chain.blocks, block = ticket % chain.blocks;
-    const int row = time * kRows + warp * S, channel = (block * 32 + lane) * V;
-    const bool mine = channel < p.channels;
-    int coming = 0;
-    if (chain.tiles > 1 && threadIdx.x == 0) coming = atomicAdd(chain.ticket, 1);
+  fetch(tile, 0);
+  for (int round = 0; tile.time >= 0; ++round) {
+    const int row = tile.time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
+    const int count = min(V, p.channels - channel);
+    if (threadIdx.x == 0)
+      coming[(round + 1) & 1] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : tiles, tiles, chain.blocks);
     const RowMap rows = map_rows<S>(p, row, active, n_seq);
-    const F bias = p.bias != nullptr && mine ? W::unpack(W::load(static_cast<const io_t*>(p.bias) + channel)) : L::all(0.0f);
+    L bias = L::all(0.0f);
+    if (LOGITS && p.bias != nullptr) {
+      const io_t* from = static_cast<const io_t*>(p.bias) + channel;
+      float b[V];
+#pragma unroll
+      for (int i = 0; i < V; ++i) b[i] = i < count ? to_f32(from[i]) * -kLog2e : 0.0f;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) bias.v[i] = make_float2(b[2 * i], b[2 * i + 1]);
+    }
+    const auto state_row = [&](int i) {  // of row i's sequence
+      const int seq = rows.seq_of(i);
+      return static_cast<long long>(p.slots != nullptr ? p.slots[seq] : seq) * p.channels + channel;
+    };
+    copies_done<0>();
+    uint2* tile_space = staged + (round & 1) * kWarps * 2 * S * 32;
+    const uint2* x = tile_space + warp * 2 * S * 32 + lane;
+    const uint2* d = x + S * 32;
 
-    // first sweep: gates and inputs into registers, and the warp's map.  A start takes its initial state into u.
-    F kept[S], u[S];
-    Piece map{L::all(1.0f), L::all(0.0f)};
+    // first sweep: the gates into registers, and the warp's map.  A start keeps the state behind it in place of its gate.
+    L kept[S];
+    Map<V> map = Map<V>::identity();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      kept[i] = D::keep(LOGITS ? L::add(W::unpack(raw_d[i]), bias) : W::unpack(raw_d[i]));
-      const F x = W::unpack(raw_x[i]);
-      u[i] = COMPLEMENT ? L::mul(D::complement(kept[i]), x) : x;
+      kept[i] = D::keep(unpack<io_t>(d[i * 32]), bias);
+      const L value = unpack<io_t>(x[i * 32]);
       if (rows.starts >> i & 1) {
-        F h = L::all(0.0f);
-        if (p.initial != nullptr && mine) {
-          const int seq = rows.seq_of(i);
-          // a plain load: the pool is written by this kernel as well
-          h = Word<float, V>::unpack(Word<float, V>::load_plain(
-              p.initial + static_cast<long long>(p.slots != nullptr ? p.slots[seq] : seq) * p.channels + channel));
-        }
-        u[i] = D::step(kept[i], h, u[i]);
-        map.b = u[i];
+        const L h = p.initial != nullptr ? load_states<V>(p.initial + state_row(i), count) : L::all(0.0f);
+        kept[i] = map.b = D::step(kept[i], h, value);
       } else {
-        map.b = D::step(kept[i], map.b, u[i]);
+        map.b = D::step(kept[i], map.b, value);
         map.a = D::fade(kept[i], map.a);
       }
     }
     pieces[warp][lane] = map;
     if (lane == 0) cut[warp] = rows.starts;
-    if (chain.tiles > 1 && threadIdx.x == 0) next_ticket[(round + 1) & 1] = coming;
     __syncthreads();
-    const int next = chain.tiles > 1 ? next_ticket[(round + 1) & 1] : tiles;
-    fetch(next);  // in flight while this tile waits and writes
+    const Tile next = coming[(round + 1) & 1];
+    fetch(next, (round + 1) & 1);  // in flight while this tile waits and writes
 
-    // the map of the warps before this one; warp 0 joins all of them for the tile
+    // the map of the warps before this one; the first warp joins all of them and publishes the tile's
+    const bool open = (cut[0] & 1) == 0;  // the tile continues a sequence
+    const int group = tile.time / kGroup, behind = tile.time % kGroup;
     bool cut_before = false;
-    Piece before{L::all(1.0f), L::all(0.0f)};
-    const int count = warp == 0 ? kWarps : warp;
-    for (int w = 0; w < count; ++w) {
-      const Piece m = pieces[w][lane];
+    Map<V> before = Map<V>::identity();
+    const int pieces_before = warp == 0 ? kWarps : warp;
+    for (int w = 0; w < pieces_before; ++w) {
+      const Map<V> m = pieces[w][lane];
       if (cut[w] != 0) {
         before = m;
         cut_before = true;
       } else {
-        before.b = L::fma(m.a, before.b, m.b);
-        before.a = L::mul(m.a, before.a);
+        before.then(m);
       }
     }
-    const bool open = (cut[0] & 1) == 0;  // the tile continues a sequence
-    if (warp == 0) {
-      const bool publish = time + 1 < chain.tiles;
-      if (publish) Chain<V>::publish(chain, block, time, {before.a, before.b}, cut_before);
-      F h = L::all(0.0f);
-      if (open) h = Chain<V>::state_before(chain, block, time);
-      carry[lane] = h;
-      if (publish && time % kGroup == kGroup - 1)
-        Chain<V>::publish_state(chain, block, time / kGroup, cut_before ? before.b : L::fma(before.a, h, before.b));
+    const bool publish = tile.time + 1 < chain.tiles;
+    if (warp == 0 && publish) Chain<V>::publish(chain, tile.block, tile.time, before, cut_before);
+    L h = L::all(0.0f);
+    if (open) {
+      if (group > 0) h = Chain<V>::look(Chain<V>::state_at(chain, tile.block, group - 1));
+      // into the place of this warp's decays, which are in registers by now
+      Chain<V>::gather(chain, tile.block, group * kGroup, behind, tile_space + S * 32, 2 * S * 32, warp, kWarps);
     }
     __syncthreads();
-    F h = carry[lane];
-    if (warp != 0) h = cut_before ? before.b : L::fma(before.a, h, before.b);
+    if (open) h = Chain<V>::join(chain, tile.block, group, tile_space + S * 32, 2 * S * 32, behind, kWarps, h);
+    if (warp == 0) {
+      if (publish && behind == kGroup - 1)
+        Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_before ? before.b : before.apply(h));
+      if (p.boundary != nullptr) store_states<V>(p.boundary + static_cast<long long>(tile.time) * p.channels + channel, h, count);
+    } else {
+      h = cut_before ? before.b : before.apply(h);
+    }
 
     // second sweep
-    if (p.boundary != nullptr && row % kTile == 0 && row < active && mine)
-      Word<float, V>::store(p.boundary + static_cast<long long>(row / kTile) * p.channels + channel, h);
     io_t* y = static_cast<io_t*>(p.y) + static_cast<long long>(row) * p.channels + channel;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      h = (rows.starts >> i & 1) ? u[i] : D::step(kept[i], h, u[i]);
-      if (mine && row + i < active) W::store(y + static_cast<long long>(i) * p.channels, h);
-      if ((rows.ends >> i & 1) && mine) {
-        const int seq = rows.seq_of(i);
-        Word<float, V>::store(p.final_state + static_cast<long long>(p.slots != nullptr ? p.slots[seq] : seq) * p.channels + channel, h);
-      }
+      h = (rows.starts >> i & 1) ? kept[i] : D::step(kept[i], h, unpack<io_t>(x[i * 32]));
+      if (row + i < active) A::store(y + static_cast<long long>(i) * p.channels, h, count);
+      if (rows.ends >> i & 1) store_states<V>(p.final_state + state_row(i), h, count);
     }
-    ticket = next;
+    tile = next;
   }
+  copies_done<0>();
 }
 
 // Decode steps (and rows of a few tokens): a thread walks V channels of one sequence, 16 bytes of a row; no chain.  The
 // state pool is most of what a step reads and writes.
 template <typename io_t, int V, bool LOGITS, bool COMPLEMENT>
 __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanParams p) {
-  using D = Decay<LOGITS, 1>;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, nullptr, 0);
     return;
@@ -168,10 +195,13 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
   if (seq >= n_seq) return;
   const int first = p.cu[seq], last = p.cu[seq + 1];
   float* state = p.final_state + static_cast<long long>(p.slots[seq]) * p.channels + channel;
+  constexpr int kPairs = (V + 1) / 2;  // V = 1 works on half a pair
+  using D = Decay<LOGITS, COMPLEMENT, 2>;
   alignas(16) io_t x[V], d[V], b[V], y[V];
-  alignas(16) float h[V];
+  alignas(16) float h[2 * kPairs];
   if constexpr (V == 1) {
     h[0] = *state;
+    h[1] = 0.0f;
     if (p.bias != nullptr) b[0] = static_cast<const io_t*>(p.bias)[channel];
   } else {
 #pragma unroll
@@ -189,11 +219,20 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
       *reinterpret_cast<uint4*>(d) = __ldcs(reinterpret_cast<const uint4*>(ds));
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const float kept = D::keep(to_f32(d[i]) + (LOGITS && p.bias != nullptr ? to_f32(b[i]) : 0.f));
-      const float value = to_f32(x[i]);
-      h[i] = D::step(kept, h[i], COMPLEMENT ? D::complement(kept) * value : value);
-      y[i] = from_f32<io_t>(h[i]);
+    for (int i = 0; i < kPairs; ++i) {
+      const auto pair = [&](const io_t* from) {
+        Lanes<2> r;
+        r.v[0] = make_float2(to_f32(from[2 * i]), V == 1 ? 0.0f : to_f32(from[V == 1 ? 0 : 2 * i + 1]));
+        return r;
+      };
+      Lanes<2> bias = Lanes<2>::all(0.0f), state_pair;
+      if (LOGITS && p.bias != nullptr) bias = mul(pair(b), Lanes<2>::all(-kLog2e));
+      state_pair.v[0] = make_float2(h[2 * i], h[2 * i + 1]);
+      state_pair = D::step(D::keep(pair(d), bias), state_pair, pair(x));
+      h[2 * i] = state_pair.v[0].x;
+      h[2 * i + 1] = state_pair.v[0].y;
+      y[2 * i] = from_f32<io_t>(h[2 * i]);
+      if constexpr (V > 1) y[2 * i + 1] = from_f32<io_t>(h[2 * i + 1]);
     }
     io_t* ys = static_cast<io_t*>(p.y) + row * p.channels + channel;
     if constexpr (V == 1) *ys = y[0];
@@ -213,189 +252,173 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
 // where c is the final state's gradient.  A tile first scans h forward from the state saved before it, keeps the
 // states in registers, and then does with g what the forward pass does with h.
 
-template <typename io_t, int V, bool LOGITS, bool COMPLEMENT>
-__global__ void __launch_bounds__(256, 2)
+template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT>
+__global__ void __launch_bounds__(kThreads, kBackwardCtas)
 gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const ChainSpace chain) {
+  constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
-  using F = typename L::type;
-  using D = Decay<LOGITS, V>;
-  using W = Word<io_t, V>;
-  struct Piece {
-    F a, b;
-  };
-  constexpr int S = 8, kWarps = 8, kRows = kWarps * S;
-  static_assert(kRows == kTile, "the forward pass saves one state for each tile of the backward pass");
-  __shared__ Piece pieces[kWarps][32], back[kWarps][32];
+  using D = Decay<LOGITS, COMPLEMENT, V>;
+  using A = Access<io_t, GRANULE>;
+  extern __shared__ uint2 staged[];  // [2 tiles][warp][x, decay or dy][S][lane]
+  __shared__ Map<V> pieces[kWarps][32];  // of h
+  __shared__ L back[kWarps][32];         // B of c's map; its A is that of h's where neither is cut
   __shared__ unsigned cut[kWarps], cut_back[kWarps];
-  __shared__ F carry[32];
-  __shared__ int next_ticket[2];
+  __shared__ Tile coming[2];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(g.dx), static_cast<io_t*>(g.ddecay), g.dinitial, p.n_seq);
     return;
   }
-  const int active = p.total, n_seq = p.n_seq;
-  const int tiles = chain.tiles * chain.blocks;
-  int round = 0, ticket = blockIdx.x;
-  if (chain.tiles > 1) {
-    if (threadIdx.x == 0) next_ticket[0] = atomicAdd(chain.ticket, 1);
-    __syncthreads();
-    ticket = next_ticket[0];
-  }
-  typename W::type raw_x[S], raw_d[S], raw_g[S];
-  const auto fetch = [&](int t) {
-    if (t >= tiles) return;
-    const int row = (chain.tiles - 1 - t / chain.blocks) * kRows + warp * S, channel = (t % chain.blocks * 32 + lane) * V;
-    const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
-    const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
-    const io_t* dy = static_cast<const io_t*>(g.dy) + static_cast<long long>(row) * p.channels + channel;
+  const int active = p.total, tiles = chain.tiles * chain.blocks;
+  const bool chained = chain.tiles > 1;
+  if (threadIdx.x == 0) coming[0] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : blockIdx.x, tiles, chain.blocks);
+  __syncthreads();
+  Tile tile = coming[0];  // counts against time
+  const auto fetch = [&](const Tile& t, int buffer) {
+    if (t.time >= 0) {
+      const int row = (chain.tiles - 1 - t.time) * kTile + warp * S, channel = (t.block * 32 + lane) * V;
+      const int count = min(V, p.channels - channel), rows = min(S, active - row);
+      const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
+      const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
+      const io_t* dy = static_cast<const io_t*>(g.dy) + static_cast<long long>(row) * p.channels + channel;
+      uint2* to = staged + (buffer * kWarps + warp) * 3 * S * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      const bool in = row + i < active && channel < p.channels;
-      raw_x[i] = in ? W::load(x + i * p.x_stride) : W::zero();
-      raw_d[i] = in ? W::load(d + i * p.decay_stride) : W::zero();
-      raw_g[i] = in ? W::load(dy + static_cast<long long>(i) * p.channels) : W::zero();
+      for (int i = 0; i < S; ++i) {
+        const int n = i < rows ? count : 0;
+        A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
+        A::stage(to + (S + i) * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
+        A::stage(to + (2 * S + i) * 32, n > 0 ? dy + static_cast<long long>(i) * p.channels : static_cast<const io_t*>(g.dy), n);
+      }
     }
+    copies_begun();
   };
-  fetch(ticket);
-  for (; ticket < tiles; ++round) {
-    const int index = ticket / chain.blocks, block = ticket % chain.blocks;  // index counts against time
-    const int time = chain.tiles - 1 - index;
-    const int row = time * kRows + warp * S, channel = (block * 32 + lane) * V;
-    const bool mine = channel < p.channels;
-    int coming = 0;
-    if (chain.tiles > 1 && threadIdx.x == 0) coming = atomicAdd(chain.ticket, 1);
-    const RowMap rows = map_rows<S>(p, row, active, n_seq);
+  fetch(tile, 0);
+  for (int round = 0; tile.time >= 0; ++round) {
+    const int index = tile.time, time = chain.tiles - 1 - index;
+    const int row = time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
+    const int count = min(V, p.channels - channel);
+    if (threadIdx.x == 0)
+      coming[(round + 1) & 1] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : tiles, tiles, chain.blocks);
+    const RowMap rows = map_rows<S>(p, row, active, p.n_seq);
+    L h = load_states<V>(p.boundary + static_cast<long long>(time) * p.channels + channel, count);
+    const auto state_of = [&](const float* states, int i) {  // of row i's sequence
+      return states != nullptr ? load_states<V>(states + static_cast<long long>(rows.seq_of(i)) * p.channels + channel, count)
+                               : L::all(0.0f);
+    };
+    copies_done<0>();
+    uint2* tile_space = staged + (round & 1) * kWarps * 3 * S * 32;
+    const uint2* x = tile_space + warp * 3 * S * 32 + lane;
+    const uint2* d = x + S * 32;
+    const uint2* dy = d + S * 32;
 
     // the warp's map of h, and its map of c: the same decays, the gradients against time
-    F kept[S], x[S], dy[S], slope[S], start[S];
-    Piece map{L::all(1.0f), L::all(0.0f)};
+    L kept[S];
+    Map<V> map = Map<V>::identity();
+    L back_b = L::all(0.0f);
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const F raw = W::unpack(raw_d[i]);
-      kept[i] = D::keep(raw);
-      slope[i] = D::slope(raw, kept[i]);
-      x[i] = W::unpack(raw_x[i]);
-      dy[i] = W::unpack(raw_g[i]);
-      const F u = COMPLEMENT ? L::mul(D::complement(kept[i]), x[i]) : x[i];
-      start[i] = L::all(0.0f);
+      kept[i] = D::keep(unpack<io_t>(d[i * 32]), L::all(0.0f));
+      const L value = unpack<io_t>(x[i * 32]);
       if (rows.starts >> i & 1) {
-        if (p.initial != nullptr && mine)
-          start[i] = Word<float, V>::unpack(Word<float, V>::load(p.initial + static_cast<long long>(rows.seq_of(i)) * p.channels + channel));
-        map.b = D::step(kept[i], start[i], u);
+        map.b = D::step(kept[i], state_of(p.initial, i), value);
       } else {
-        map.b = D::step(kept[i], map.b, u);
-        map.a = D::fade(kept[i], map.a);
+        map.b = D::step(kept[i], map.b, value);
       }
+      map.a = D::fade(kept[i], map.a);  // of all rows: it counts only where no bound lies between them
     }
-    Piece map_back{L::all(1.0f), L::all(0.0f)};
 #pragma unroll
-    for (int i = S - 1; i >= 0; --i) {
-      if (rows.ends >> i & 1) {
-        const F last = g.dfinal != nullptr && mine
-                           ? Word<float, V>::unpack(Word<float, V>::load(g.dfinal + static_cast<long long>(rows.seq_of(i)) * p.channels + channel))
-                           : L::all(0.0f);
-        dy[i] = L::add(dy[i], last);
-        map_back.b = D::fade(kept[i], dy[i]);
-      } else {
-        map_back.b = D::fade(kept[i], L::add(dy[i], map_back.b));
-        map_back.a = D::fade(kept[i], map_back.a);
-      }
-    }
-    F h = L::all(0.0f);
-    if (mine)
-      h = Word<float, V>::unpack(Word<float, V>::load(p.boundary + static_cast<long long>(time) * p.channels + channel));
+    for (int i = S - 1; i >= 0; --i)
+      back_b = D::fade(kept[i], add(unpack<io_t>(dy[i * 32]), (rows.ends >> i & 1) ? state_of(g.dfinal, i) : back_b));
     pieces[warp][lane] = map;
-    back[warp][lane] = map_back;
+    back[warp][lane] = back_b;
     if (lane == 0) {
       cut[warp] = rows.starts;
       cut_back[warp] = rows.ends;
     }
-    if (chain.tiles > 1 && threadIdx.x == 0) next_ticket[(round + 1) & 1] = coming;
     __syncthreads();
-    const int next = chain.tiles > 1 ? next_ticket[(round + 1) & 1] : tiles;
-    fetch(next);
+    const Tile next = coming[(round + 1) & 1];
+    fetch(next, (round + 1) & 1);
 
-    for (int w = 0; w < warp; ++w) {
-      const Piece m = pieces[w][lane];
-      h = cut[w] != 0 ? m.b : L::fma(m.a, h, m.b);
-    }
+    // the map of the warps behind this one; the last warp joins all of them and publishes the tile's
+    const bool open = index > 0 && (cut_back[kWarps - 1] >> (S - 1) & 1) == 0;  // the last row's sequence goes on
+    const int group = index / kGroup, before = index % kGroup;
     bool cut_behind = false;
-    Piece behind{L::all(1.0f), L::all(0.0f)};  // of the warps behind this one; the last warp joins all of them
+    Map<V> behind = Map<V>::identity();
     const int stop = warp == kWarps - 1 ? 0 : warp + 1;
     for (int w = kWarps - 1; w >= stop; --w) {
-      const Piece m = back[w][lane];
+      const Map<V> m{pieces[w][lane].a, back[w][lane]};
       if (cut_back[w] != 0) {
         behind = m;
         cut_behind = true;
       } else {
-        behind.b = L::fma(m.a, behind.b, m.b);
-        behind.a = L::mul(m.a, behind.a);
+        behind.then(m);
       }
     }
-    if (warp == kWarps - 1) {
-      const bool publish = index + 1 < chain.tiles;
-      if (publish) Chain<V>::publish(chain, block, index, {behind.a, behind.b}, cut_behind);
-      F c = L::all(0.0f);
-      // the tile's last row in use continues into the next tile
-      if (index > 0 && (rows.ends >> (S - 1) & 1) == 0) c = Chain<V>::state_before(chain, block, index);
-      carry[lane] = c;
-      if (publish && index % kGroup == kGroup - 1)
-        Chain<V>::publish_state(chain, block, index / kGroup, cut_behind ? behind.b : L::fma(behind.a, c, behind.b));
+    const bool publish = index + 1 < chain.tiles;
+    if (warp == kWarps - 1 && publish) Chain<V>::publish(chain, tile.block, index, behind, cut_behind);
+    L c = L::all(0.0f);
+    // what ddecay needs of the states: the state before every row, less its input (complement)
+    for (int w = 0; w < warp; ++w) {
+      const Map<V> m = pieces[w][lane];
+      h = cut[w] != 0 ? m.b : m.apply(h);
     }
-    __syncthreads();
-    F c = carry[lane];
-    if (warp != kWarps - 1) c = cut_behind ? behind.b : L::fma(behind.a, c, behind.b);
-
-    // states before every row
-    F states[S];
+    L states[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      if (rows.starts >> i & 1) h = start[i];
-      states[i] = h;
-      h = D::step(kept[i], h, COMPLEMENT ? L::mul(D::complement(kept[i]), x[i]) : x[i]);
+      if (rows.starts >> i & 1) h = state_of(p.initial, i);
+      const L value = unpack<io_t>(x[i * 32]);
+      states[i] = COMPLEMENT ? minus(h, value) : h;
+      h = D::step(kept[i], h, value);
     }
+    if (open) {
+      if (group > 0) c = Chain<V>::look(Chain<V>::state_at(chain, tile.block, group - 1));
+      // into the place of this warp's inputs, which are used up
+      __syncwarp();
+      Chain<V>::gather(chain, tile.block, group * kGroup, before, tile_space, 3 * S * 32, warp, kWarps);
+    }
+    __syncthreads();
+    if (open) c = Chain<V>::join(chain, tile.block, group, tile_space, 3 * S * 32, before, kWarps, c);
+    if (warp == kWarps - 1) {
+      if (publish && before == kGroup - 1)
+        Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_behind ? behind.b : behind.apply(c));
+    } else {
+      c = cut_behind ? behind.b : behind.apply(c);
+    }
+
     io_t* dx = static_cast<io_t*>(g.dx) + static_cast<long long>(row) * p.channels + channel;
     io_t* dd = static_cast<io_t*>(g.ddecay) + static_cast<long long>(row) * p.channels + channel;
 #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-      const F grad = (rows.ends >> i & 1) ? dy[i] : L::add(dy[i], c);
+      const L grad = add(unpack<io_t>(dy[i * 32]), (rows.ends >> i & 1) ? state_of(g.dfinal, i) : c);
       c = D::fade(kept[i], grad);
-      if (mine && row + i < active) {
-        W::store(dx + static_cast<long long>(i) * p.channels, COMPLEMENT ? L::mul(D::complement(kept[i]), grad) : grad);
-        // d / d(1 - rho): the input (complement) less the state before
-        const F source = L::fma(states[i], L::all(-1.0f), COMPLEMENT ? x[i] : L::all(0.0f));
-        W::store(dd + static_cast<long long>(i) * p.channels, L::mul(L::mul(grad, source), slope[i]));
+      if (row + i < active) {
+        A::store(dx + static_cast<long long>(i) * p.channels, D::input_grad(kept[i], grad), count);
+        L drho = mul(grad, states[i]);
+        if constexpr (LOGITS) drho = mul(drho, D::slope(D::sigmoid(unpack<io_t>(d[i * 32]), L::all(0.0f)), kept[i]));
+        A::store(dd + static_cast<long long>(i) * p.channels, drho, count);
       }
-      if ((rows.starts >> i & 1) && mine && g.dinitial != nullptr)
-        Word<float, V>::store(g.dinitial + static_cast<long long>(rows.seq_of(i)) * p.channels + channel, c);
+      if ((rows.starts >> i & 1) && g.dinitial != nullptr)
+        store_states<V>(g.dinitial + static_cast<long long>(rows.seq_of(i)) * p.channels + channel, c, count);
     }
-    ticket = next;
+    tile = next;
   }
+  copies_done<0>();
 }
 
 // ---- launches
 
-constexpr int kForwardWarps = 16, kForwardRows = 8;  // a warp's rows
-
-long long round_up(long long n, long long to) { return (n + to - 1) / to * to; }
-
-// Where the chain lives in the workspace; the flags and the counter come first and are cleared by every call.
-ChainSpace chain_space(void* workspace, int total, int channels, int rows, int lanes, long long* clear_bytes, long long* bytes) {
+// Where the chain lives in the workspace.  All of it is filled with kEmpty by every call that uses it.
+ChainSpace chain_space(void* workspace, int total, int channels, int lanes, long long* bytes) {
   ChainSpace c{};
-  c.tiles = (total + rows - 1) / rows;
+  c.tiles = (total + kTile - 1) / kTile;
   c.groups = (c.tiles + kGroup - 1) / kGroup;
   c.blocks = (channels + lanes - 1) / lanes;
   char* base = static_cast<char*>(workspace);
-  const long long tile_flags = 4ll * c.tiles * c.blocks, group_flags = 4ll * c.groups * c.blocks;
+  const long long maps = 8ll * c.tiles * c.blocks * lanes, states = 4ll * c.groups * c.blocks * lanes;
   c.ticket = reinterpret_cast<int*>(base);
-  c.tile_flags = reinterpret_cast<int*>(base + 16);
-  c.group_flags = reinterpret_cast<int*>(base + 16 + tile_flags);
-  *clear_bytes = 16 + tile_flags + group_flags;
-  const long long maps = round_up(*clear_bytes, 256), states = maps + 8ll * c.tiles * c.blocks * lanes;
-  c.maps = reinterpret_cast<float*>(base + maps);
-  c.states = reinterpret_cast<float*>(base + states);
-  *bytes = c.tiles > 1 ? states + 4ll * c.groups * c.blocks * lanes : 0;
+  c.maps = reinterpret_cast<float*>(base + 256);
+  c.states = reinterpret_cast<float*>(base + 256 + maps);
+  *bytes = c.tiles > 1 ? 256 + maps + states : 0;
   return c;
 }
 
@@ -447,40 +470,51 @@ template <typename F> void with_modes(int decay_mode, int input_mode, F f) {
   }
 }
 
-// Calls f with the token type and the channels of a lane as compile-time constants: pairs of 16-bit channels (one
-// 128-byte row piece for a warp) where `pairs` allows them, else single channels (fp32: 128 bytes as well).
-template <typename F> void with_type(int io_dtype, bool pairs, F f) {
-  using one = std::integral_constant<int, 1>;
+// Calls f with the token type and the largest access that fits everything as compile-time constants.
+template <typename F> void with_type(int io_dtype, int granule, F f) {
   using two = std::integral_constant<int, 2>;
-  if (io_dtype == FRWKV_IO_FP32) f(float{}, one{});
-  else if (io_dtype == FRWKV_IO_BF16 && pairs) f(__nv_bfloat16{}, two{});
-  else if (io_dtype == FRWKV_IO_BF16) f(__nv_bfloat16{}, one{});
-  else if (pairs) f(__half{}, two{});
-  else f(__half{}, one{});
+  using four = std::integral_constant<int, 4>;
+  using eight = std::integral_constant<int, 8>;
+  if (io_dtype == FRWKV_IO_FP32) granule == 8 ? f(float{}, eight{}) : f(float{}, four{});
+  else if (io_dtype == FRWKV_IO_BF16) granule == 8 ? f(__nv_bfloat16{}, eight{}) : granule == 4 ? f(__nv_bfloat16{}, four{}) : f(__nv_bfloat16{}, two{});
+  else granule == 8 ? f(__half{}, eight{}) : granule == 4 ? f(__half{}, four{}) : f(__half{}, two{});
 }
 
-bool pairs_fit(const GatedScanParams& p) {
-  return p.channels % 2 == 0 && p.x_stride % 2 == 0 && p.decay_stride % 2 == 0 && multiple_of(4, {p.x, p.decay, p.bias, p.y}) &&
-         multiple_of(8, {p.initial, p.final_state, p.boundary});
+// The bytes of a token row that one access may move: 8 where the channels, the strides and all starts allow it.
+int granule_of(const GatedScanParams& p, int io_dtype, std::initializer_list<const void*> rows) {
+  const int element = io_dtype == FRWKV_IO_FP32 ? 4 : 2;
+  for (int granule = 8; granule > element; granule /= 2) {
+    const int n = granule / element;
+    if (p.channels % n == 0 && p.x_stride % n == 0 && p.decay_stride % n == 0 && multiple_of(granule, rows)) return granule;
+  }
+  return element;
+}
+
+// Launches a chained kernel: fills the chain's space, as many CTAs as are resident at most.
+template <typename K, typename... Args>
+int launch_chained(K kernel, int lanes, int tensors, int ctas, const GatedScanParams& p, void* workspace, cudaStream_t s,
+                   const char* what, Args... args) {
+  long long bytes;
+  const ChainSpace chain = chain_space(workspace, p.total, p.channels, lanes, &bytes);
+  const int shared = 2 * tensors * kTile * 256;  // two tiles of 256-byte rows
+  cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+  if (error == cudaSuccess && chain.tiles > 1) error = cudaMemsetAsync(workspace, 0xff, bytes, s);
+  if (error != cudaSuccess) return fail(FRWKV_ERR_CUDA, "%s: preparing the launch: %s", what, cudaGetErrorString(error));
+  const long long tiles = static_cast<long long>(chain.tiles) * chain.blocks, resident = static_cast<long long>(ctas) * sm_count();
+  const unsigned grid = static_cast<unsigned>(chain.tiles > 1 && tiles > resident ? resident : tiles);
+  kernel<<<grid, kThreads, shared, s>>>(p, args..., chain);
+  return check_launch(what);
 }
 
 int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, void* workspace, void* stream) {
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t cleared = cudaSuccess;
-  with_type(io_dtype, pairs_fit(p), [&](auto io, auto v) {
+  int rc = FRWKV_OK;
+  with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
-      long long clear_bytes, bytes;
-      const ChainSpace chain =
-          chain_space(workspace, p.total, p.channels, kForwardWarps * kForwardRows, 32 * v(), &clear_bytes, &bytes);
-      if (chain.tiles > 1) cleared = cudaMemsetAsync(workspace, 0, clear_bytes, s);
-      const long long tiles = static_cast<long long>(chain.tiles) * chain.blocks, resident = 2ll * sm_count();
-      const unsigned grid = static_cast<unsigned>(chain.tiles > 1 && tiles > resident ? resident : tiles);
-      gated_scan_forward_kernel<decltype(io), v(), kForwardRows, kForwardWarps, logits(), complement()>
-          <<<grid, kForwardWarps * 32, 0, s>>>(p, chain);
+      rc = launch_chained(gated_scan_forward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), 2,
+                          kForwardCtas, p, workspace, static_cast<cudaStream_t>(stream), "gated_scan_forward_kernel");
     });
   });
-  if (cleared != cudaSuccess) return fail(FRWKV_ERR_CUDA, "gated_scan: clearing the workspace: %s", cudaGetErrorString(cleared));
-  return check_launch("gated_scan_forward_kernel");
+  return rc;
 }
 
 int run_steps(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, void* stream) {
@@ -506,11 +540,10 @@ int run_steps(const GatedScanParams& p, int io_dtype, int decay_mode, int input_
 
 extern "C" size_t frwkv_sm100_gated_scan_workspace_bytes(int total_tokens, int channels) {
   if (total_tokens <= 0 || channels <= 0) return 0;
-  // the backward pass has the smaller tiles; the wider of single channels and pairs
-  long long clear_bytes, single, pairs;
-  frwkv::chain_space(nullptr, total_tokens, channels, FRWKV_GATED_SCAN_TILE, 32, &clear_bytes, &single);
-  frwkv::chain_space(nullptr, total_tokens, channels, FRWKV_GATED_SCAN_TILE, 64, &clear_bytes, &pairs);
-  return static_cast<size_t>(single > pairs ? single : pairs);
+  long long wide, narrow;  // channel blocks of fp32 and of 16-bit tokens
+  frwkv::chain_space(nullptr, total_tokens, channels, 64, &wide);
+  frwkv::chain_space(nullptr, total_tokens, channels, 128, &narrow);
+  return static_cast<size_t>(wide > narrow ? wide : narrow);
 }
 
 extern "C" int frwkv_sm100_gated_scan(
@@ -568,19 +601,12 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
                           nullptr, const_cast<float*>(boundary), nullptr, n_seq, total_tokens, channels,
                           total_tokens / n_seq};
   const GatedScanGrads g{dy, dfinal, dx, ddecay, dinitial};
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  cudaError_t cleared = cudaSuccess;
-  const bool pairs = pairs_fit(p) && multiple_of(4, {dy, dx, ddecay}) && multiple_of(8, {dfinal, dinitial});
-  with_type(io_dtype, pairs, [&](auto io, auto v) {
+  int rc = FRWKV_OK;
+  with_type(io_dtype, granule_of(p, io_dtype, {x, decay, dy, dx, ddecay}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
-      long long clear_bytes, bytes;
-      const ChainSpace chain = chain_space(workspace, total_tokens, channels, kTile, 32 * v(), &clear_bytes, &bytes);
-      if (chain.tiles > 1) cleared = cudaMemsetAsync(workspace, 0, clear_bytes, s);
-      const long long tiles = static_cast<long long>(chain.tiles) * chain.blocks, resident = 2ll * sm_count();
-      const unsigned grid = static_cast<unsigned>(chain.tiles > 1 && tiles > resident ? resident : tiles);
-      gated_scan_backward_kernel<decltype(io), v(), logits(), complement()><<<grid, 256, 0, s>>>(p, g, chain);
+      rc = launch_chained(gated_scan_backward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), 3,
+                          kBackwardCtas, p, workspace, static_cast<cudaStream_t>(stream), "gated_scan_backward_kernel", g);
     });
   });
-  if (cleared != cudaSuccess) return fail(FRWKV_ERR_CUDA, "gated_scan: clearing the workspace: %s", cudaGetErrorString(cleared));
-  return check_launch("gated_scan_backward_kernel");
+  return rc;
 }
