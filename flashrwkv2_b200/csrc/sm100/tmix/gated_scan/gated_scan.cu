@@ -13,10 +13,7 @@ namespace {
 
 constexpr int kTile = FRWKV_GATED_SCAN_TILE;
 constexpr int S = 8, kWarps = 8, kThreads = kWarps * 32;
-#ifndef FC
-#define FC 3
-#endif
-constexpr int kForwardCtas = FC, kBackwardCtas = 2;  // per SM: 64 KB of staging each, 96 KB backward
+constexpr int kForwardCtas = 2, kBackwardCtas = 2;  // per SM: 96 KB of staging each
 static_assert(S * kWarps == kTile, "the forward pass saves one state for each tile of the backward pass");
 
 // NaN in every row that the call would write (fail-closed), by the whole grid.
@@ -49,18 +46,25 @@ __device__ __forceinline__ Tile tile_of(int ticket, int tiles, int blocks) {
 __device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" : : : "memory"); }
 template <int LEFT> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" : : "n"(LEFT) : "memory"); }
 
+// Barrier of a CTA whose warps have taken different ways.
+__device__ __forceinline__ void tile_barrier() { asm volatile("bar.sync 1, %0;" : : "n"(kThreads + 32) : "memory"); }
+
 // ---- forward
 
+// Eight warps sweep, a ninth keeps the chain.  While the eight do the first sweep of tile n + 1, the ninth publishes
+// tile n's map and finds the state before it, so a tile's second sweep comes one tile after its first and nobody waits for
+// another CTA; the gates of two tiles are in registers.  One barrier a tile.
 template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT>
-__global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_kernel(const GatedScanParams p, const ChainSpace chain) {
+__global__ void __launch_bounds__(kThreads + 32, kForwardCtas) gated_scan_forward_kernel(const GatedScanParams p, const ChainSpace chain) {
   constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
   using A = Access<io_t, GRANULE>;
-  extern __shared__ uint2 staged[];  // [2 tiles][warp][x or decay][S][lane]
-  __shared__ Map<V> pieces[kWarps][32];
-  __shared__ unsigned cut[kWarps];
-  __shared__ Tile coming[2];
+  // [3 tiles][warp][x or decay][S][lane]; a warp's decays make room for its map and for the state before its rows
+  extern __shared__ uint2 staged[];
+  constexpr int kTensor = S * 32, kWarpSpace = 2 * kTensor, kTileSpace = kWarps * kWarpSpace;
+  __shared__ unsigned cuts[2][kWarps];
+  __shared__ Tile ring[4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, p.boundary != nullptr ? p.final_state : nullptr, p.n_seq);
@@ -70,31 +74,88 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_ker
   const int n_seq = p.status != nullptr ? p.status[2] : p.n_seq;
   const int tiles = (active + kTile - 1) / kTile * chain.blocks;  // of the rows in use
   const bool chained = chain.tiles > 1;
-  if (threadIdx.x == 0) coming[0] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : blockIdx.x, tiles, chain.blocks);
+  const bool more = chained && tiles > static_cast<int>(gridDim.x);  // than one tile for each CTA
+  if (threadIdx.x == 0) {  // one after the other: a CTA's tickets ascend
+    for (int i = 0; i < 3; ++i) {
+      int ticket = i == 0 ? blockIdx.x : tiles;
+      if (i == 0 ? chained : more) ticket = atomicAdd(chain.ticket, 1) + 1;
+      ring[i] = tile_of(ticket, tiles, chain.blocks);
+    }
+  }
   __syncthreads();
-  Tile tile = coming[0];
+  const auto map_space = [&](int buffer, int w) { return reinterpret_cast<Map<V>*>(staged + buffer * kTileSpace + w * kWarpSpace + kTensor) + lane; };
+  const auto state_space = [&](int buffer, int w) {
+    return reinterpret_cast<L*>(staged + buffer * kTileSpace + w * kWarpSpace + kTensor + kTensor / 2) + lane;
+  };
+
+  if (warp == kWarps) {
+    tile_barrier();
+    for (int n = 0, buffer = 0;; ++n, buffer = buffer == 2 ? 0 : buffer + 1) {
+      const Tile tile = ring[n & 3];
+      if (tile.time < 0) break;
+      int ticket = tiles;
+      if (more && lane == 0) ticket = atomicAdd(chain.ticket, 1) + 1;
+      const unsigned* cut = cuts[n & 1];
+      const int group = tile.time / kGroup, behind = tile.time % kGroup;
+      const bool publish = tile.time + 1 < chain.tiles;
+      Map<V> all = Map<V>::identity();
+      bool cut_inside = false;
+      if (publish) {
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const Map<V> m = *map_space(buffer, w);
+          if (cut[w] != 0) {
+            all = m;
+            cut_inside = true;
+          } else {
+            all.then(m);
+          }
+        }
+        Chain<V>::publish(chain, tile.block, tile.time, all, cut_inside);
+      }
+      L h = L::all(0.0f);
+      if ((cut[0] & 1) == 0) h = Chain<V>::state_before(chain, tile.block, group, behind);  // the tile continues a sequence
+      if (publish && behind == kGroup - 1)
+        Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_inside ? all.b : all.apply(h));
+      const int channel = (tile.block * 32 + lane) * V;
+      if (p.boundary != nullptr)
+        store_states<V>(p.boundary + static_cast<long long>(tile.time) * p.channels + channel, h, min(V, p.channels - channel));
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        *state_space(buffer, w) = h;
+        const Map<V> m = *map_space(buffer, w);
+        h = cut[w] != 0 ? m.b : m.apply(h);
+      }
+      if (lane == 0) ring[(n + 3) & 3] = tile_of(ticket, tiles, chain.blocks);
+      tile_barrier();
+    }
+    return;
+  }
+
   const auto fetch = [&](const Tile& t, int buffer) {
     if (t.time >= 0) {
       const int row = t.time * kTile + warp * S, channel = (t.block * 32 + lane) * V;
       const int count = min(V, p.channels - channel), rows = min(S, active - row);
       const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
       const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
-      uint2* to = staged + (buffer * kWarps + warp) * 2 * S * 32 + lane;
+      uint2* to = staged + buffer * kTileSpace + warp * kWarpSpace + lane;
 #pragma unroll
       for (int i = 0; i < S; ++i) {
         const int n = i < rows ? count : 0;
         A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
-        A::stage(to + (S + i) * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
+        A::stage(to + kTensor + i * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
       }
     }
     copies_begun();
   };
-  fetch(tile, 0);
-  for (int round = 0; tile.time >= 0; ++round) {
+  const auto state_row = [&](const RowMap& rows, int i, int channel) {  // of row i's sequence
+    const int seq = rows.seq_of(i);
+    return static_cast<long long>(p.slots != nullptr ? p.slots[seq] : seq) * p.channels + channel;
+  };
+  // First sweep: the gates into registers, and the warp's map.  A start keeps the state behind it in place of its gate.
+  const auto first_sweep = [&](const Tile& tile, int n, int buffer, L (&kept)[S]) {
     const int row = tile.time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
     const int count = min(V, p.channels - channel);
-    if (threadIdx.x == 0)
-      coming[(round + 1) & 1] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : tiles, tiles, chain.blocks);
     const RowMap rows = map_rows<S>(p, row, active, n_seq);
     L bias = L::all(0.0f);
     if (LOGITS && p.bias != nullptr) {
@@ -105,78 +166,70 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_ker
 #pragma unroll
       for (int i = 0; i < V / 2; ++i) bias.v[i] = make_float2(b[2 * i], b[2 * i + 1]);
     }
-    const auto state_row = [&](int i) {  // of row i's sequence
-      const int seq = rows.seq_of(i);
-      return static_cast<long long>(p.slots != nullptr ? p.slots[seq] : seq) * p.channels + channel;
-    };
-    copies_done<0>();
-    uint2* tile_space = staged + (round & 1) * kWarps * 2 * S * 32;
-    const uint2* x = tile_space + warp * 2 * S * 32 + lane;
-    const uint2* d = x + S * 32;
-
-    // first sweep: the gates into registers, and the warp's map.  A start keeps the state behind it in place of its gate.
-    L kept[S];
+    const uint2* x = staged + buffer * kTileSpace + warp * kWarpSpace + lane;
     Map<V> map = Map<V>::identity();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      kept[i] = D::keep(unpack<io_t>(d[i * 32]), bias);
+      kept[i] = D::keep(unpack<io_t>(x[kTensor + i * 32]), bias);
       const L value = unpack<io_t>(x[i * 32]);
       if (rows.starts >> i & 1) {
-        const L h = p.initial != nullptr ? load_states<V>(p.initial + state_row(i), count) : L::all(0.0f);
+        const L h = p.initial != nullptr ? load_states<V>(p.initial + state_row(rows, i, channel), count) : L::all(0.0f);
         kept[i] = map.b = D::step(kept[i], h, value);
       } else {
         map.b = D::step(kept[i], map.b, value);
         map.a = D::fade(kept[i], map.a);
       }
     }
-    pieces[warp][lane] = map;
-    if (lane == 0) cut[warp] = rows.starts;
-    __syncthreads();
-    const Tile next = coming[(round + 1) & 1];
-    fetch(next, (round + 1) & 1);  // in flight while this tile waits and writes
-
-    // the map of the warps before this one; the first warp joins all of them and publishes the tile's
-    const bool open = (cut[0] & 1) == 0;  // the tile continues a sequence
-    const int group = tile.time / kGroup, behind = tile.time % kGroup;
-    bool cut_before = false;
-    Map<V> before = Map<V>::identity();
-    const int pieces_before = warp == 0 ? kWarps : warp;
-    for (int w = 0; w < pieces_before; ++w) {
-      const Map<V> m = pieces[w][lane];
-      if (cut[w] != 0) {
-        before = m;
-        cut_before = true;
-      } else {
-        before.then(m);
-      }
-    }
-    const bool publish = tile.time + 1 < chain.tiles;
-    if (warp == 0 && publish) Chain<V>::publish(chain, tile.block, tile.time, before, cut_before);
-    L h = L::all(0.0f);
-    if (open) {
-      if (group > 0) h = Chain<V>::look(Chain<V>::state_at(chain, tile.block, group - 1));
-      // into the place of this warp's decays, which are in registers by now
-      Chain<V>::gather(chain, tile.block, group * kGroup, behind, tile_space + S * 32, 2 * S * 32, warp, kWarps);
-    }
-    __syncthreads();
-    if (open) h = Chain<V>::join(chain, tile.block, group, tile_space + S * 32, 2 * S * 32, behind, kWarps, h);
-    if (warp == 0) {
-      if (publish && behind == kGroup - 1)
-        Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_before ? before.b : before.apply(h));
-      if (p.boundary != nullptr) store_states<V>(p.boundary + static_cast<long long>(tile.time) * p.channels + channel, h, count);
-    } else {
-      h = cut_before ? before.b : before.apply(h);
-    }
-
-    // second sweep
+    __syncwarp();  // every lane has read its decays
+    *map_space(buffer, warp) = map;
+    if (lane == 0) cuts[n & 1][warp] = rows.starts;
+    return rows;
+  };
+  const auto second_sweep = [&](const Tile& tile, const RowMap& rows, int buffer, const L (&kept)[S]) {
+    const int row = tile.time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
+    const int count = min(V, p.channels - channel);
+    const uint2* x = staged + buffer * kTileSpace + warp * kWarpSpace + lane;
+    L h = *state_space(buffer, warp);
     io_t* y = static_cast<io_t*>(p.y) + static_cast<long long>(row) * p.channels + channel;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       h = (rows.starts >> i & 1) ? kept[i] : D::step(kept[i], h, unpack<io_t>(x[i * 32]));
       if (row + i < active) A::store(y + static_cast<long long>(i) * p.channels, h, count);
-      if (rows.ends >> i & 1) store_states<V>(p.final_state + state_row(i), h, count);
+      if (rows.ends >> i & 1) store_states<V>(p.final_state + state_row(rows, i, channel), h, count);
     }
+    __syncwarp();  // every lane has read its state: the space may be filled again
+  };
+  L kept_even[S], kept_odd[S];
+  RowMap rows_even, rows_odd;
+  Tile tile = ring[0];
+  fetch(tile, 0);
+  fetch(ring[1], 1);
+  fetch(ring[2], 2);
+  if (tile.time >= 0) {
+    copies_done<2>();
+    rows_even = first_sweep(tile, 0, 0, kept_even);
+  }
+  tile_barrier();
+  // one tile: the first sweep of the next, the barrier, the second sweep of this one, its space to the tile after next
+  int n = 0, buffer = 0;
+  const auto advance = [&](const RowMap& rows, const L (&kept)[S], RowMap& next_rows, L (&next_kept)[S]) {
+    const Tile next = ring[(n + 1) & 3];
+    const int next_buffer = buffer == 2 ? 0 : buffer + 1;
+    if (next.time >= 0) {
+      copies_done<1>();
+      next_rows = first_sweep(next, n + 1, next_buffer, next_kept);
+    }
+    tile_barrier();
+    second_sweep(tile, rows, buffer, kept);
+    fetch(ring[(n + 3) & 3], buffer);
     tile = next;
+    buffer = next_buffer;
+    ++n;
+  };
+  while (tile.time >= 0) {
+    advance(rows_even, kept_even, rows_odd, kept_odd);
+    if (tile.time < 0) break;
+    advance(rows_odd, kept_odd, rows_even, kept_even);
   }
   copies_done<0>();
 }
@@ -261,6 +314,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   using A = Access<io_t, GRANULE>;
   extern __shared__ uint2 staged[];  // [2 tiles][warp][x, decay or dy][S][lane]
   __shared__ Map<V> pieces[kWarps][32];  // of h
+  __shared__ L carry[32];
   __shared__ L back[kWarps][32];         // B of c's map; its A is that of h's where neither is cut
   __shared__ unsigned cut[kWarps], cut_back[kWarps];
   __shared__ Tile coming[2];
@@ -306,8 +360,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
                                : L::all(0.0f);
     };
     copies_done<0>();
-    uint2* tile_space = staged + (round & 1) * kWarps * 3 * S * 32;
-    const uint2* x = tile_space + warp * 3 * S * 32 + lane;
+    const uint2* x = staged + ((round & 1) * kWarps + warp) * 3 * S * 32 + lane;
     const uint2* d = x + S * 32;
     const uint2* dy = d + S * 32;
 
@@ -370,14 +423,12 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
       states[i] = COMPLEMENT ? minus(h, value) : h;
       h = D::step(kept[i], h, value);
     }
-    if (open) {
-      if (group > 0) c = Chain<V>::look(Chain<V>::state_at(chain, tile.block, group - 1));
-      // into the place of this warp's inputs, which are used up
-      __syncwarp();
-      Chain<V>::gather(chain, tile.block, group * kGroup, before, tile_space, 3 * S * 32, warp, kWarps);
+    if (warp == kWarps - 1) {
+      if (open) c = Chain<V>::state_before(chain, tile.block, group, before);
+      carry[lane] = c;
     }
     __syncthreads();
-    if (open) c = Chain<V>::join(chain, tile.block, group, tile_space, 3 * S * 32, before, kWarps, c);
+    c = carry[lane];
     if (warp == kWarps - 1) {
       if (publish && before == kGroup - 1)
         Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_behind ? behind.b : behind.apply(c));
@@ -492,17 +543,17 @@ int granule_of(const GatedScanParams& p, int io_dtype, std::initializer_list<con
 
 // Launches a chained kernel: fills the chain's space, as many CTAs as are resident at most.
 template <typename K, typename... Args>
-int launch_chained(K kernel, int lanes, int tensors, int ctas, const GatedScanParams& p, void* workspace, cudaStream_t s,
+int launch_chained(K kernel, int lanes, int threads, int tensors, int ctas, const GatedScanParams& p, void* workspace, cudaStream_t s,
                    const char* what, Args... args) {
   long long bytes;
   const ChainSpace chain = chain_space(workspace, p.total, p.channels, lanes, &bytes);
-  const int shared = 2 * tensors * kTile * 256;  // two tiles of 256-byte rows
+  const int shared = tensors * kTile * 256;  // 256-byte rows
   cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
   if (error == cudaSuccess && chain.tiles > 1) error = cudaMemsetAsync(workspace, 0xff, bytes, s);
   if (error != cudaSuccess) return fail(FRWKV_ERR_CUDA, "%s: preparing the launch: %s", what, cudaGetErrorString(error));
   const long long tiles = static_cast<long long>(chain.tiles) * chain.blocks, resident = static_cast<long long>(ctas) * sm_count();
   const unsigned grid = static_cast<unsigned>(chain.tiles > 1 && tiles > resident ? resident : tiles);
-  kernel<<<grid, kThreads, shared, s>>>(p, args..., chain);
+  kernel<<<grid, threads, shared, s>>>(p, args..., chain);
   return check_launch(what);
 }
 
@@ -510,7 +561,7 @@ int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int inpu
   int rc = FRWKV_OK;
   with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
-      rc = launch_chained(gated_scan_forward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), 2,
+      rc = launch_chained(gated_scan_forward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), kThreads + 32, 3 * 2,
                           kForwardCtas, p, workspace, static_cast<cudaStream_t>(stream), "gated_scan_forward_kernel");
     });
   });
@@ -604,7 +655,7 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
   int rc = FRWKV_OK;
   with_type(io_dtype, granule_of(p, io_dtype, {x, decay, dy, dx, ddecay}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
-      rc = launch_chained(gated_scan_backward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), 3,
+      rc = launch_chained(gated_scan_backward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), kThreads, 2 * 3,
                           kBackwardCtas, p, workspace, static_cast<cudaStream_t>(stream), "gated_scan_backward_kernel", g);
     });
   });

@@ -334,34 +334,39 @@ template <int V> struct Chain {
     put(to + 32 * V, m.b);
   }
   static __device__ __forceinline__ bool is_cut(const L& a) { return __float_as_uint(a.v[0].x) == kCut; }  // all lanes agree
-  // The maps of the n < kGroup tiles before one in its group into shared memory, by all warps of the CTA: map i by warp
-  // i % warps, into that warp's own space (`spaces` are `pitch` words of 8 bytes apart).
-  static __device__ __forceinline__ Map<V>* slot(uint2* spaces, int pitch, int i, int warps) {
-    return reinterpret_cast<Map<V>*>(spaces + i % warps * pitch) + i / warps * 32 + (threadIdx.x & 31);
-  }
-  static __device__ __forceinline__ void gather(const ChainSpace& c, int block, int first, int n, uint2* spaces, int pitch, int warp, int warps) {
-    for (int i = warp; i < n; i += warps) {
-      const float* from = map_at(c, block, first + i);
-      const L a = look(from), b = look(from + 32 * V);
-      *slot(spaces, pitch, i, warps) = Map<V>{wait(from, a), wait(from + 32 * V, b)};
-    }
-  }
-  // The state before a tile: the gathered maps behind the state that the group before left.
-  static __device__ __forceinline__ L join(const ChainSpace& c, int block, int group, uint2* spaces, int pitch, int n, int warps, const L& early) {
+  // The state before a tile, by one warp: the maps of the n < kGroup tiles before it in its group behind the state that
+  // the group before left.  All maps are asked for in batches before the first is waited for.
+  static __device__ __forceinline__ L state_before(const ChainSpace& c, int block, int group, int n) {
+    L state = L::all(0.0f);
+    if (group > 0) state = look(state_at(c, block, group - 1));
     Map<V> all = Map<V>::identity();
     bool cut = false;
-    for (int i = 0; i < n; ++i) {
-      const Map<V> m = *slot(spaces, pitch, i, warps);
-      if (is_cut(m.a)) {
-        all.b = m.b;
-        cut = true;
-      } else {
-        all.then(m);
+    constexpr int kBatch = 8;
+    for (int base = 0; base < n; base += kBatch) {
+      const float* from = map_at(c, block, group * kGroup + base);
+      Map<V> m[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float* at = from + (base + i < n ? i : 0) * 64 * V;
+        m[i].a = look(at);
+        m[i].b = look(at + 32 * V);
+      }
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (base + i >= n) break;
+        m[i].a = wait(from + i * 64 * V, m[i].a);
+        m[i].b = wait(from + i * 64 * V + 32 * V, m[i].b);
+        if (is_cut(m[i].a)) {
+          all.b = m[i].b;
+          cut = true;
+        } else {
+          all.then(m[i]);
+        }
       }
     }
     if (cut) return all.b;
     if (group == 0) return L::all(__int_as_float(0x7fffffff));  // no sequence starts at row 0: not valid
-    return all.apply(wait(state_at(c, block, group - 1), early));
+    return all.apply(wait(state_at(c, block, group - 1), state));
   }
 };
 
