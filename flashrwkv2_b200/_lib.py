@@ -33,7 +33,6 @@ SYMBOLS = (
     "frwkv_sm100_wkv7_prefill_readout",
     "frwkv_sm100_wkv7_pretrain_forward",
     "frwkv_sm100_wkv7_pretrain_backward",
-    "frwkv_sm100_gated_scan_workspace_bytes",
     "frwkv_sm100_gated_scan",
     "frwkv_sm100_gated_scan_train_forward",
     "frwkv_sm100_gated_scan_train_backward",
@@ -95,14 +94,12 @@ def declare(lib: ctypes.CDLL) -> ctypes.CDLL:
     lib.frwkv_sm100_wkv7_pretrain_backward.restype = ci
     lib.frwkv_sm100_wkv7_pretrain_backward.argtypes = [vp] * 15 + [ci, ci, ci, vp]
     ll = ctypes.c_longlong
-    lib.frwkv_sm100_gated_scan_workspace_bytes.restype = sz
-    lib.frwkv_sm100_gated_scan_workspace_bytes.argtypes = [ci, ci]
     lib.frwkv_sm100_gated_scan.restype = ci
-    lib.frwkv_sm100_gated_scan.argtypes = [vp] * 5 + [ll, vp, ll, vp, vp] + [ci] * 7 + [vp, sz, vp]
+    lib.frwkv_sm100_gated_scan.argtypes = [vp] * 5 + [ll, vp, ll, vp, vp] + [ci] * 7 + [vp]
     lib.frwkv_sm100_gated_scan_train_forward.restype = ci
-    lib.frwkv_sm100_gated_scan_train_forward.argtypes = [vp] * 3 + [ll, vp, ll] + [vp] * 4 + [ci] * 6 + [vp, sz, vp]
+    lib.frwkv_sm100_gated_scan_train_forward.argtypes = [vp] * 3 + [ll, vp, ll] + [vp] * 4 + [ci] * 7 + [vp]
     lib.frwkv_sm100_gated_scan_train_backward.restype = ci
-    lib.frwkv_sm100_gated_scan_train_backward.argtypes = [vp] * 3 + [ll, vp, ll] + [vp] * 7 + [ci] * 6 + [vp, sz, vp]
+    lib.frwkv_sm100_gated_scan_train_backward.argtypes = [vp] * 3 + [ll, vp, ll] + [vp] * 7 + [ci] * 7 + [vp]
     lib.frwkv_sm100_token_logprobs.restype = ci
     lib.frwkv_sm100_token_logprobs.argtypes = [vp] + [ll] * 4 + [vp, ci, ll] + [ci, ci, cf, ci] + [vp] * 6
     lib.frwkv_sm100_token_logprobs_backward.restype = ci

@@ -1,4 +1,4 @@
-// Torch-facing shim of the gated scan: argument checks (TypeError / ValueError), output and workspace tensors, the
+// Torch-facing shim of the gated scan: argument checks (TypeError / ValueError), output tensors, the
 // metadata ticket of the packed forms; raw pointers and torch's current stream go to the C ABI.  No arithmetic here.
 #include "bindings.h"
 
@@ -65,19 +65,6 @@ void check_fp32(const torch::Tensor& t, at::IntArrayRef shape, const char* name,
   need_value(t.is_contiguous(), std::string(name) + " must be contiguous");
 }
 
-struct Workspace {
-  torch::Tensor tensor;
-  void* data;
-  size_t bytes;
-};
-
-Workspace make_workspace(const torch::Tensor& x, const RowsShape& s) {
-  const size_t bytes = frwkv_sm100_gated_scan_workspace_bytes(static_cast<int>(s.total), static_cast<int>(s.channels));
-  if (bytes == 0) return Workspace{torch::Tensor(), nullptr, 0};
-  auto tensor = torch::empty({static_cast<int64_t>(bytes)}, x.options().dtype(torch::kUInt8));
-  return Workspace{tensor, tensor.data_ptr(), bytes};
-}
-
 void* optional_pointer(const std::optional<torch::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
 torch::Tensor tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const torch::Tensor& state_indices,
@@ -113,12 +100,11 @@ torch::Tensor tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const t
   const c10::cuda::CUDAGuard guard(x.device());
   const auto meta = resolve_metadata(query_start_loc, state_indices, state, x, validated_metadata, max_seqlen);
   auto y = torch::empty(x.sizes(), x.options());
-  const Workspace work = make_workspace(x, s);
   check_abi(frwkv_sm100_gated_scan(
       meta.cu.data_ptr<int>(), meta.slots.data_ptr<int>(), meta.status.data_ptr<int>(), state.data_ptr<float>(),
       x.data_ptr(), s.x_stride, decay_logits.data_ptr(), s.decay_stride, optional_pointer(decay_bias), y.data_ptr(),
       static_cast<int>(state_indices.numel()), static_cast<int>(s.total), static_cast<int>(s.channels), io_code(x), mode,
-      input, static_cast<int>(meta.max_seqlen), work.data, work.bytes,
+      input, static_cast<int>(meta.max_seqlen),
       at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
   return y;
 }
@@ -157,14 +143,13 @@ py::tuple pretrain_tmix_gated_scan_forward(const torch::Tensor& x, const torch::
   auto y = torch::empty(x.sizes(), x.options());
   const auto fp32 = x.options().dtype(torch::kFloat32);
   auto final_state = torch::empty({n, s.channels}, fp32);
-  auto boundary = torch::empty({(s.total + FRWKV_GATED_SCAN_TILE - 1) / FRWKV_GATED_SCAN_TILE, s.channels}, fp32);
-  const Workspace work = make_workspace(x, s);
+  auto boundary = torch::empty({s.total / FRWKV_GATED_SCAN_SAVED_ROWS + n, s.channels}, fp32);
   check_abi(frwkv_sm100_gated_scan_train_forward(
       static_cast<const int32_t*>(optional_pointer(cu)), static_cast<const int32_t*>(optional_pointer(status)),
       x.data_ptr(), s.x_stride, decay_logits.data_ptr(), s.decay_stride,
       static_cast<const float*>(optional_pointer(initial_state)), y.data_ptr(), final_state.data_ptr<float>(),
       boundary.data_ptr<float>(), static_cast<int>(n), static_cast<int>(s.total), static_cast<int>(s.channels),
-      io_code(x), mode, input, work.data, work.bytes, at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
+      io_code(x), mode, input, -1, at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
   return py::make_tuple(y, final_state, boundary, cu, status);
 }
 
@@ -180,7 +165,7 @@ py::tuple pretrain_tmix_gated_scan_backward(const torch::Tensor& x, const torch:
   need_type(grad_output.scalar_type() == x.scalar_type(), "grad_output must have x's dtype");
   need_value(grad_output.sizes() == x.sizes() && grad_output.is_contiguous() && grad_output.device() == x.device(),
              "grad_output must be contiguous with x's shape and device");
-  check_fp32(boundary, {(s.total + FRWKV_GATED_SCAN_TILE - 1) / FRWKV_GATED_SCAN_TILE, s.channels}, "boundary", "[tiles,C]");
+  check_fp32(boundary, {s.total / FRWKV_GATED_SCAN_SAVED_ROWS + n, s.channels}, "boundary", "[saved rows,C]");
   if (initial_state.has_value()) check_fp32(*initial_state, {n, s.channels}, "initial_state", "[N,C]");
   if (grad_final.has_value()) check_fp32(*grad_final, {n, s.channels}, "grad_final", "[N,C]");
   const c10::cuda::CUDAGuard guard(x.device());
@@ -188,14 +173,13 @@ py::tuple pretrain_tmix_gated_scan_backward(const torch::Tensor& x, const torch:
   auto ddecay = torch::empty(x.sizes(), x.options());
   Optional dinitial;
   if (initial_state.has_value()) dinitial = torch::empty_like(*initial_state);
-  const Workspace work = make_workspace(x, s);
   check_abi(frwkv_sm100_gated_scan_train_backward(
       static_cast<const int32_t*>(optional_pointer(cu)), static_cast<const int32_t*>(optional_pointer(status)),
       x.data_ptr(), s.x_stride, decay_logits.data_ptr(), s.decay_stride,
       static_cast<const float*>(optional_pointer(initial_state)), boundary.data_ptr<float>(), grad_output.data_ptr(),
       static_cast<const float*>(optional_pointer(grad_final)), dx.data_ptr(), ddecay.data_ptr(),
       static_cast<float*>(optional_pointer(dinitial)), static_cast<int>(n), static_cast<int>(s.total),
-      static_cast<int>(s.channels), io_code(x), mode, input, work.data, work.bytes,
+      static_cast<int>(s.channels), io_code(x), mode, input, -1,
       at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
   return py::make_tuple(dx, ddecay, dinitial);
 }

@@ -1,20 +1,30 @@
 // Gated scan: in-place serving operator and training forward / backward (see gated_scan.cuh for the arithmetic).
 //
-// Rows are cut into tiles of 64 consecutive tokens by 256 bytes of channels, without regard to sequences: a start inside a
-// tile cuts the recurrence there.  A warp owns 8 tokens, a lane 8 bytes of channels.  The tokens come through shared
-// memory (cp.async, the next tile's while this one is worked on); a first sweep computes the gates into registers and
-// gives the warp's affine map, the CTA joins the maps of its warps, the chain (gated_scan.cuh) gives the state before the
-// tile, a second sweep writes the rows.  So the tokens are read once and the outputs written once, time is split over the
-// whole GPU even for one sequence, and a batch of ragged sequences is as regular as a dense one.
+// A cluster of CTAs (one, where there is enough to do) walks one sequence over 64 bytes of channels, the state carried from
+// step to step.  In a step each CTA takes a tile of 256 tokens: a warp 32 of them, a lane 8 tokens of 8 bytes of channels.
+// The tokens come through shared memory (cp.async, the next tile's while this one is worked on).  A first sweep computes the
+// gates into registers and gives each lane an affine map of the state, h -> a h + b, over its 8 tokens; the maps are joined
+// over the warp's four lane groups (shuffles), its warps (shared memory) and the cluster's CTAs (distributed shared
+// memory), always in the same order; a second sweep over the registers writes the rows.  So the tokens are read once and
+// the outputs written once, and nothing waits for anything outside its cluster.
 #include "gated_scan.cuh"
+
+#include <cooperative_groups.h>
+
+#include <algorithm>
 
 namespace frwkv {
 namespace {
 
-constexpr int kTile = FRWKV_GATED_SCAN_TILE;
+namespace cg = cooperative_groups;
+
 constexpr int S = 8, kWarps = 8, kThreads = kWarps * 32;
-constexpr int kForwardCtas = 2, kBackwardCtas = 2;  // per SM: 96 KB of staging each
-static_assert(S * kWarps == kTile, "the forward pass saves one state for each tile of the backward pass");
+constexpr int kLanes = 8, kGroups = 32 / kLanes;  // lanes along the channels, groups of them along time
+constexpr int kWarpRows = kGroups * S, kTile = kWarps * kWarpRows;
+constexpr int kForwardCtas = 3, kBackwardCtas = 2;  // per SM: 64 KB and 96 KB of staging each
+constexpr int kMaxCluster = 8;
+constexpr int kShortRows = 16;  // sequences of at most this many tokens are served by the step kernel
+static_assert(kWarpRows == kSavedRows, "the backward pass loads a state for every warp");
 
 // NaN in every row that the call would write (fail-closed), by the whole grid.
 template <typename io_t>
@@ -27,211 +37,202 @@ __device__ void fill_rows_nan(const GatedScanParams& p, io_t* rows, io_t* more_r
     fill_output_nan<float>(states, nullptr, static_cast<long long>(n_states) * p.channels, self, threads);
 }
 
-// Persistent CTAs take tiles in order and learn their next one a tile ahead; with one tile of rows there is no chain
-// and no counter.
-__device__ __forceinline__ int take_ticket(const ChainSpace& chain) { return atomicAdd(chain.ticket, 1) + 1; }
+__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" : : : "memory"); }
+__device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group 0;" : : : "memory"); }
 
-// A CTA's tiles: time tile, channel block.  Persistent CTAs take tiles in order and learn their next one a tile ahead.
-struct Tile {
-  int time, block;  // time < 0: none left
+// The work of a cluster: a block of channels of up to 32 consecutive sequences, one after the other.
+struct Unit {
+  unsigned left;   // bit i: sequence first_seq + i is still to do
+  int first_seq;
+  int channel;     // of this lane
+
+  // Next sequence, or -1.
+  __device__ __forceinline__ int next() {
+    if (left == 0) return -1;
+    const int i = __ffs(left) - 1;
+    left &= left - 1;
+    return first_seq + i;
+  }
 };
 
-// Which tile a ticket stands for; `tiles` of them are in use.
-__device__ __forceinline__ Tile tile_of(int ticket, int tiles, int blocks) {
-  if (ticket >= tiles) return Tile{-1, 0};
-  const int time = ticket / blocks;
-  return Tile{time, ticket - time * blocks};
+struct Grid {
+  int blocks;    // channel blocks
+  int per_unit;  // sequences of a unit
+  int cluster;   // CTAs of a cluster
+};
+
+__device__ __forceinline__ int row_begin(const GatedScanParams& p, int seq) { return p.cu != nullptr ? p.cu[seq] : seq * p.seq_len; }
+
+template <int V> __device__ __forceinline__ Unit unit_of(const GatedScanParams& p, const Grid& g, int unit, int n_seq) {
+  const int lane = threadIdx.x & 31, chunk = unit / g.blocks;
+  Unit u;
+  u.first_seq = chunk * g.per_unit;
+  u.channel = ((unit - chunk * g.blocks) * kLanes + lane % kLanes) * V;
+  const int seq = u.first_seq + lane;
+  const bool mine = lane < g.per_unit && seq < n_seq && row_begin(p, seq + 1) - row_begin(p, seq) > p.longer_than;
+  u.left = __ballot_sync(0xffffffffu, mine);
+  return u;
 }
 
-__device__ __forceinline__ void copies_begun() { asm volatile("cp.async.commit_group;" : : : "memory"); }
-template <int LEFT> __device__ __forceinline__ void copies_done() { asm volatile("cp.async.wait_group %0;" : : "n"(LEFT) : "memory"); }
+// A CTA's tile: rows [row, row + kTile) of a sequence, which has `left` rows from there on (none, behind its end).
+struct Tile {
+  int seq;    // < 0: there is none
+  int begin;  // first row of the sequence
+  int at;     // of the tile, in the sequence
+  int len;    // of the sequence
+};
 
-// Barrier of a CTA whose warps have taken different ways.
-__device__ __forceinline__ void tile_barrier() { asm volatile("bar.sync 1, %0;" : : "n"(kThreads + 32) : "memory"); }
+template <int V> struct Scan {
+  using L = Lanes<V>;
+
+  // Inclusive join of the maps of a warp's lane groups, in their order; returns the map before this lane's rows.
+  static __device__ __forceinline__ Map<V> join_groups(Map<V>& m) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int d = kLanes; d < 32; d *= 2) {
+      Map<V> before{shuffle_up(m.a, d), shuffle_up(m.b, d)};
+      if (lane >= d) {
+        before.then(m);
+        m = before;
+      }
+    }
+    Map<V> before{shuffle_up(m.a, kLanes), shuffle_up(m.b, kLanes)};
+    return lane >= kLanes ? before : Map<V>::identity();
+  }
+};
+
+// Joins the CTAs of a cluster: each writes its map into everyone's shared memory (slots[rank]), a cluster barrier, and each
+// applies the maps of the ranks before it.  Returns the state before this CTA's tile and moves `carry` behind the cluster's.
+template <int V>
+__device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Map<V> (*slots)[kLanes], Lanes<V>& carry) {
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp < ranks && lane < kLanes) cluster.map_shared_rank(&slots[rank][0], warp)[lane] = cta;
+  cluster.sync();
+  Lanes<V> mine = carry;
+  for (int r = 0; r < ranks; ++r) {
+    if (r == rank) mine = carry;
+    carry = slots[r][lane % kLanes].apply(carry);
+  }
+  return mine;
+}
 
 // ---- forward
 
-// Eight warps sweep, a ninth keeps the chain.  While the eight do the first sweep of tile n + 1, the ninth publishes
-// tile n's map and finds the state before it, so a tile's second sweep comes one tile after its first and nobody waits for
-// another CTA; the gates of two tiles are in registers.  One barrier a tile.
-template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT>
-__global__ void __launch_bounds__(kThreads + 32, kForwardCtas) gated_scan_forward_kernel(const GatedScanParams p, const ChainSpace chain) {
+template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
   using A = Access<io_t, GRANULE>;
-  // [3 tiles][warp][x or decay][S][lane]; a warp's decays make room for its map and for the state before its rows
-  extern __shared__ uint2 staged[];
-  constexpr int kTensor = S * 32, kWarpSpace = 2 * kTensor, kTileSpace = kWarps * kWarpSpace;
-  __shared__ unsigned cuts[2][kWarps];
-  __shared__ Tile ring[4];
+  extern __shared__ uint2 staged[];  // [2 tiles][x or decay][warp][S][lane]
+  constexpr int kTensor = kWarps * S * 32, kTileSpace = 2 * kTensor;
+  __shared__ Map<V> pieces[2][kWarps][kLanes], slots[2][CLUSTER ? kMaxCluster : 1][kLanes];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, p.boundary != nullptr ? p.final_state : nullptr, p.n_seq);
     return;
   }
-  const int active = p.status != nullptr ? p.status[1] : p.total;
+  if constexpr (CLUSTER) cg::this_cluster().sync();  // everyone's shared memory is there before it is written to
   const int n_seq = p.status != nullptr ? p.status[2] : p.n_seq;
-  const int tiles = (active + kTile - 1) / kTile * chain.blocks;  // of the rows in use
-  const bool chained = chain.tiles > 1;
-  const bool more = chained && tiles > static_cast<int>(gridDim.x);  // than one tile for each CTA
-  if (threadIdx.x == 0) {  // one after the other: a CTA's tickets ascend
-    for (int i = 0; i < 3; ++i) {
-      int ticket = i == 0 ? blockIdx.x : tiles;
-      if (i == 0 ? chained : more) ticket = atomicAdd(chain.ticket, 1) + 1;
-      ring[i] = tile_of(ticket, tiles, chain.blocks);
-    }
-  }
-  __syncthreads();
-  const auto map_space = [&](int buffer, int w) { return reinterpret_cast<Map<V>*>(staged + buffer * kTileSpace + w * kWarpSpace + kTensor) + lane; };
-  const auto state_space = [&](int buffer, int w) {
-    return reinterpret_cast<L*>(staged + buffer * kTileSpace + w * kWarpSpace + kTensor + kTensor / 2) + lane;
+  const int ranks = CLUSTER ? grid.cluster : 1, rank = CLUSTER ? static_cast<int>(blockIdx.x) % ranks : 0;
+  Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, n_seq);
+  const int channel = unit.channel, count = min(V, p.channels - channel);
+  const auto first_tile = [&](int seq) {
+    if (seq < 0) return Tile{-1, 0, 0, 0};
+    const int begin = row_begin(p, seq);
+    return Tile{seq, begin, rank * kTile, row_begin(p, seq + 1) - begin};
   };
-
-  if (warp == kWarps) {
-    tile_barrier();
-    for (int n = 0, buffer = 0;; ++n, buffer = buffer == 2 ? 0 : buffer + 1) {
-      const Tile tile = ring[n & 3];
-      if (tile.time < 0) break;
-      int ticket = tiles;
-      if (more && lane == 0) ticket = atomicAdd(chain.ticket, 1) + 1;
-      const unsigned* cut = cuts[n & 1];
-      const int group = tile.time / kGroup, behind = tile.time % kGroup;
-      const bool publish = tile.time + 1 < chain.tiles;
-      Map<V> all = Map<V>::identity();
-      bool cut_inside = false;
-      if (publish) {
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const Map<V> m = *map_space(buffer, w);
-          if (cut[w] != 0) {
-            all = m;
-            cut_inside = true;
-          } else {
-            all.then(m);
-          }
-        }
-        Chain<V>::publish(chain, tile.block, tile.time, all, cut_inside);
-      }
-      L h = L::all(0.0f);
-      if ((cut[0] & 1) == 0) h = Chain<V>::state_before(chain, tile.block, group, behind);  // the tile continues a sequence
-      if (publish && behind == kGroup - 1)
-        Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_inside ? all.b : all.apply(h));
-      const int channel = (tile.block * 32 + lane) * V;
-      if (p.boundary != nullptr)
-        store_states<V>(p.boundary + static_cast<long long>(tile.time) * p.channels + channel, h, min(V, p.channels - channel));
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        *state_space(buffer, w) = h;
-        const Map<V> m = *map_space(buffer, w);
-        h = cut[w] != 0 ? m.b : m.apply(h);
-      }
-      if (lane == 0) ring[(n + 3) & 3] = tile_of(ticket, tiles, chain.blocks);
-      tile_barrier();
-    }
-    return;
-  }
-
+  const auto tile_after = [&](const Tile& t) {
+    const int at = t.at + ranks * kTile;
+    return at - rank * kTile < t.len ? Tile{t.seq, t.begin, at, t.len} : first_tile(unit.next());
+  };
+  const int own = warp * kWarpRows + lane / kLanes * S;  // this lane's first row in a tile
   const auto fetch = [&](const Tile& t, int buffer) {
-    if (t.time >= 0) {
-      const int row = t.time * kTile + warp * S, channel = (t.block * 32 + lane) * V;
-      const int count = min(V, p.channels - channel), rows = min(S, active - row);
+    if (t.seq >= 0) {
+      const int left = t.len - t.at - own, row = t.begin + t.at + own;
       const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
       const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
-      uint2* to = staged + buffer * kTileSpace + warp * kWarpSpace + lane;
+      uint2* to = staged + buffer * kTileSpace + warp * S * 32 + lane;
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        const int n = i < rows ? count : 0;
+        const int n = i < left ? count : 0;
         A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
         A::stage(to + kTensor + i * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
       }
     }
     copies_begun();
   };
-  const auto state_row = [&](const RowMap& rows, int i, int channel) {  // of row i's sequence
-    const int seq = rows.seq_of(i);
+  const auto state_row = [&](int seq) {
     return static_cast<long long>(p.slots != nullptr ? p.slots[seq] : seq) * p.channels + channel;
   };
-  // First sweep: the gates into registers, and the warp's map.  A start keeps the state behind it in place of its gate.
-  const auto first_sweep = [&](const Tile& tile, int n, int buffer, L (&kept)[S]) {
-    const int row = tile.time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
-    const int count = min(V, p.channels - channel);
-    const RowMap rows = map_rows<S>(p, row, active, n_seq);
-    L bias = L::all(0.0f);
-    if (LOGITS && p.bias != nullptr) {
-      const io_t* from = static_cast<const io_t*>(p.bias) + channel;
-      float b[V];
+  const auto initial_state = [&](const Tile& t) {
+    return t.seq >= 0 && p.initial != nullptr ? load_states<V>(p.initial + state_row(t.seq), count) : L::all(0.0f);
+  };
+  L bias = L::all(0.0f);
+  if (LOGITS && p.bias != nullptr) {
+    const io_t* from = static_cast<const io_t*>(p.bias) + channel;
+    float b[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) b[i] = i < count ? to_f32(from[i]) * -kLog2e : 0.0f;
+    for (int i = 0; i < V; ++i) b[i] = i < count ? to_f32(from[i]) * -kLog2e : 0.0f;
 #pragma unroll
-      for (int i = 0; i < V / 2; ++i) bias.v[i] = make_float2(b[2 * i], b[2 * i + 1]);
-    }
-    const uint2* x = staged + buffer * kTileSpace + warp * kWarpSpace + lane;
+    for (int i = 0; i < V / 2; ++i) bias.v[i] = make_float2(b[2 * i], b[2 * i + 1]);
+  }
+  Tile tile = first_tile(unit.next());
+  fetch(tile, 0);
+  L carry = initial_state(tile);
+  for (int round = 0; tile.seq >= 0; ++round) {
+    const int buffer = round & 1;
+    const Tile next = tile_after(tile);
+    copies_done();
+    const uint2* x = staged + buffer * kTileSpace + warp * S * 32 + lane;
+
+    // first sweep: the gates into registers, and the map of this lane's rows
+    L kept[S];
     Map<V> map = Map<V>::identity();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       kept[i] = D::keep(unpack<io_t>(x[kTensor + i * 32]), bias);
-      const L value = unpack<io_t>(x[i * 32]);
-      if (rows.starts >> i & 1) {
-        const L h = p.initial != nullptr ? load_states<V>(p.initial + state_row(rows, i, channel), count) : L::all(0.0f);
-        kept[i] = map.b = D::step(kept[i], h, value);
-      } else {
-        map.b = D::step(kept[i], map.b, value);
-        map.a = D::fade(kept[i], map.a);
+      map.b = D::step(kept[i], map.b, unpack<io_t>(x[i * 32]));
+      map.a = D::fade(kept[i], map.a);
+    }
+    fetch(next, buffer ^ 1);  // in flight while this tile is joined and written
+    const Map<V> before = Scan<V>::join_groups(map);
+    if (lane >= 32 - kLanes) pieces[buffer][warp][lane % kLanes] = map;
+    __syncthreads();
+
+    // the state before this warp's rows, and behind the tile
+    L h = carry;
+    if constexpr (CLUSTER) {
+      Map<V> cta = pieces[buffer][0][lane % kLanes];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w][lane % kLanes]);
+      h = join_cluster<V>(cta, slots[buffer], carry);
+      for (int w = 0; w < warp; ++w) h = pieces[buffer][w][lane % kLanes].apply(h);
+    } else {
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) h = carry;
+        carry = pieces[buffer][w][lane % kLanes].apply(carry);
       }
     }
-    __syncwarp();  // every lane has read its decays
-    *map_space(buffer, warp) = map;
-    if (lane == 0) cuts[n & 1][warp] = rows.starts;
-    return rows;
-  };
-  const auto second_sweep = [&](const Tile& tile, const RowMap& rows, int buffer, const L (&kept)[S]) {
-    const int row = tile.time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
-    const int count = min(V, p.channels - channel);
-    const uint2* x = staged + buffer * kTileSpace + warp * kWarpSpace + lane;
-    L h = *state_space(buffer, warp);
-    io_t* y = static_cast<io_t*>(p.y) + static_cast<long long>(row) * p.channels + channel;
+    const int left = tile.len - tile.at - own;
+    if (p.boundary != nullptr && lane < kLanes && left > 0)
+      store_states<V>(p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel, h, count);
+    h = before.apply(h);
+    if (next.seq != tile.seq) carry = initial_state(next);
+
+    // second sweep
+    io_t* y = static_cast<io_t*>(p.y) + static_cast<long long>(tile.begin + tile.at + own) * p.channels + channel;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      h = (rows.starts >> i & 1) ? kept[i] : D::step(kept[i], h, unpack<io_t>(x[i * 32]));
-      if (row + i < active) A::store(y + static_cast<long long>(i) * p.channels, h, count);
-      if (rows.ends >> i & 1) store_states<V>(p.final_state + state_row(rows, i, channel), h, count);
+      h = D::step(kept[i], h, unpack<io_t>(x[i * 32]));
+      if (i < left) A::store(y + static_cast<long long>(i) * p.channels, h, count);
+      if (i + 1 == left) store_states<V>(p.final_state + state_row(tile.seq), h, count);
     }
-    __syncwarp();  // every lane has read its state: the space may be filled again
-  };
-  L kept_even[S], kept_odd[S];
-  RowMap rows_even, rows_odd;
-  Tile tile = ring[0];
-  fetch(tile, 0);
-  fetch(ring[1], 1);
-  fetch(ring[2], 2);
-  if (tile.time >= 0) {
-    copies_done<2>();
-    rows_even = first_sweep(tile, 0, 0, kept_even);
-  }
-  tile_barrier();
-  // one tile: the first sweep of the next, the barrier, the second sweep of this one, its space to the tile after next
-  int n = 0, buffer = 0;
-  const auto advance = [&](const RowMap& rows, const L (&kept)[S], RowMap& next_rows, L (&next_kept)[S]) {
-    const Tile next = ring[(n + 1) & 3];
-    const int next_buffer = buffer == 2 ? 0 : buffer + 1;
-    if (next.time >= 0) {
-      copies_done<1>();
-      next_rows = first_sweep(next, n + 1, next_buffer, next_kept);
-    }
-    tile_barrier();
-    second_sweep(tile, rows, buffer, kept);
-    fetch(ring[(n + 3) & 3], buffer);
     tile = next;
-    buffer = next_buffer;
-    ++n;
-  };
-  while (tile.time >= 0) {
-    advance(rows_even, kept_even, rows_odd, kept_odd);
-    if (tile.time < 0) break;
-    advance(rows_odd, kept_odd, rows_even, kept_even);
   }
-  copies_done<0>();
 }
 
 // Decode steps (and rows of a few tokens): a thread walks V channels of one sequence, 16 bytes of a row; no chain.  The
@@ -247,6 +248,7 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
   const int seq = static_cast<int>(at / per_row), channel = static_cast<int>(at % per_row) * V;
   if (seq >= n_seq) return;
   const int first = p.cu[seq], last = p.cu[seq + 1];
+  if (last - first > p.longer_than) return;  // the other kernel's
   float* state = p.final_state + static_cast<long long>(p.slots[seq]) * p.channels + channel;
   constexpr int kPairs = (V + 1) / 2;  // V = 1 works on half a pair
   using D = Decay<LOGITS, COMPLEMENT, 2>;
@@ -301,177 +303,157 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
 
 // ---- backward
 //
-// With c_t = rho_t g_t the same recurrence runs against time: g_t = dy_t + c_{t+1}, cut behind a sequence's last token,
-// where c is the final state's gradient.  A tile first scans h forward from the state saved before it, keeps the
-// states in registers, and then does with g what the forward pass does with h.
+// With c_t = rho_t g_t the same recurrence runs against time: g_t = dy_t + c_{t+1}, and c behind the last token is the final
+// state's gradient.  Steps go from the end of a sequence to its start and rank 0 of a cluster takes the last of a step's
+// tiles; inside a tile warps, lane groups and rows are counted from its end, so that all joins are those of the forward
+// pass.  The states come from those that the forward pass saved before every warp's rows.
 
-template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT>
+template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas)
-gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const ChainSpace chain) {
+gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
   using A = Access<io_t, GRANULE>;
-  extern __shared__ uint2 staged[];  // [2 tiles][warp][x, decay or dy][S][lane]
-  __shared__ Map<V> pieces[kWarps][32];  // of h
-  __shared__ L carry[32];
-  __shared__ L back[kWarps][32];         // B of c's map; its A is that of h's where neither is cut
-  __shared__ unsigned cut[kWarps], cut_back[kWarps];
-  __shared__ Tile coming[2];
+  extern __shared__ uint2 staged[];  // [2 tiles][x, decay or dy][warp][S][lane]
+  constexpr int kTensor = kWarps * S * 32, kTileSpace = 3 * kTensor;
+  __shared__ Map<V> pieces[2][kWarps][kLanes], slots[2][CLUSTER ? kMaxCluster : 1][kLanes];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(g.dx), static_cast<io_t*>(g.ddecay), g.dinitial, p.n_seq);
     return;
   }
-  const int active = p.total, tiles = chain.tiles * chain.blocks;
-  const bool chained = chain.tiles > 1;
-  if (threadIdx.x == 0) coming[0] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : blockIdx.x, tiles, chain.blocks);
-  __syncthreads();
-  Tile tile = coming[0];  // counts against time
+  if constexpr (CLUSTER) cg::this_cluster().sync();
+  const int ranks = CLUSTER ? grid.cluster : 1, rank = CLUSTER ? static_cast<int>(blockIdx.x) % ranks : 0;
+  Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, p.n_seq);
+  const int channel = unit.channel, count = min(V, p.channels - channel);
+  const int step_rows = ranks * kTile;
+  const auto first_tile = [&](int seq) {
+    if (seq < 0) return Tile{-1, 0, 0, 0};
+    const int begin = row_begin(p, seq), len = row_begin(p, seq + 1) - begin;
+    return Tile{seq, begin, (len - 1) / step_rows * step_rows + (ranks - 1 - rank) * kTile, len};
+  };
+  const auto tile_after = [&](const Tile& t) {
+    return t.at >= step_rows ? Tile{t.seq, t.begin, t.at - step_rows, t.len} : first_tile(unit.next());
+  };
+  const int own = (kWarps - 1 - warp) * kWarpRows + (kGroups - 1 - lane / kLanes) * S;
   const auto fetch = [&](const Tile& t, int buffer) {
-    if (t.time >= 0) {
-      const int row = (chain.tiles - 1 - t.time) * kTile + warp * S, channel = (t.block * 32 + lane) * V;
-      const int count = min(V, p.channels - channel), rows = min(S, active - row);
+    if (t.seq >= 0) {
+      const int left = t.len - t.at - own, row = t.begin + t.at + own;
       const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
       const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
       const io_t* dy = static_cast<const io_t*>(g.dy) + static_cast<long long>(row) * p.channels + channel;
-      uint2* to = staged + (buffer * kWarps + warp) * 3 * S * 32 + lane;
+      uint2* to = staged + buffer * kTileSpace + warp * S * 32 + lane;
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        const int n = i < rows ? count : 0;
+        const int n = i < left ? count : 0;
         A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
-        A::stage(to + (S + i) * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
-        A::stage(to + (2 * S + i) * 32, n > 0 ? dy + static_cast<long long>(i) * p.channels : static_cast<const io_t*>(g.dy), n);
+        A::stage(to + kTensor + i * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
+        A::stage(to + 2 * kTensor + i * 32, n > 0 ? dy + static_cast<long long>(i) * p.channels : static_cast<const io_t*>(g.dy), n);
       }
     }
     copies_begun();
   };
+  const auto final_grad = [&](const Tile& t) {
+    return t.seq >= 0 && g.dfinal != nullptr ? load_states<V>(g.dfinal + static_cast<long long>(t.seq) * p.channels + channel, count)
+                                             : L::all(0.0f);
+  };
+  Tile tile = first_tile(unit.next());
   fetch(tile, 0);
-  for (int round = 0; tile.time >= 0; ++round) {
-    const int index = tile.time, time = chain.tiles - 1 - index;
-    const int row = time * kTile + warp * S, channel = (tile.block * 32 + lane) * V;
-    const int count = min(V, p.channels - channel);
-    if (threadIdx.x == 0)
-      coming[(round + 1) & 1] = tile_of(chained ? atomicAdd(chain.ticket, 1) + 1 : tiles, tiles, chain.blocks);
-    const RowMap rows = map_rows<S>(p, row, active, p.n_seq);
-    L h = load_states<V>(p.boundary + static_cast<long long>(time) * p.channels + channel, count);
-    const auto state_of = [&](const float* states, int i) {  // of row i's sequence
-      return states != nullptr ? load_states<V>(states + static_cast<long long>(rows.seq_of(i)) * p.channels + channel, count)
-                               : L::all(0.0f);
-    };
-    copies_done<0>();
-    const uint2* x = staged + ((round & 1) * kWarps + warp) * 3 * S * 32 + lane;
-    const uint2* d = x + S * 32;
-    const uint2* dy = d + S * 32;
+  L carry = final_grad(tile);
+  for (int round = 0; tile.seq >= 0; ++round) {
+    const int buffer = round & 1, left = tile.len - tile.at - own;
+    const Tile next = tile_after(tile);
+    // the state before this warp's rows, where it has any
+    const int warp_at = tile.at + (kWarps - 1 - warp) * kWarpRows;
+    const L saved = warp_at < tile.len
+                        ? load_states<V>(p.boundary + saved_row(tile.seq, tile.begin, warp_at) * p.channels + channel, count)
+                        : L::all(0.0f);
+    copies_done();
+    const uint2* x = staged + buffer * kTileSpace + warp * S * 32 + lane;
+    const uint2* d = x + kTensor;
+    const uint2* dy = d + kTensor;
 
-    // the warp's map of h, and its map of c: the same decays, the gradients against time
+    // first sweep: the gates, and the maps of h (rows in time) and c (against it).  Rows behind the sequence's end leave c as
+    // it is.
     L kept[S];
-    Map<V> map = Map<V>::identity();
-    L back_b = L::all(0.0f);
+    Map<V> map = Map<V>::identity(), back = map;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       kept[i] = D::keep(unpack<io_t>(d[i * 32]), L::all(0.0f));
-      const L value = unpack<io_t>(x[i * 32]);
-      if (rows.starts >> i & 1) {
-        map.b = D::step(kept[i], state_of(p.initial, i), value);
-      } else {
-        map.b = D::step(kept[i], map.b, value);
-      }
-      map.a = D::fade(kept[i], map.a);  // of all rows: it counts only where no bound lies between them
+      map.b = D::step(kept[i], map.b, unpack<io_t>(x[i * 32]));
+      if (i < left) map.a = D::fade(kept[i], map.a);
     }
 #pragma unroll
-    for (int i = S - 1; i >= 0; --i)
-      back_b = D::fade(kept[i], add(unpack<io_t>(dy[i * 32]), (rows.ends >> i & 1) ? state_of(g.dfinal, i) : back_b));
-    pieces[warp][lane] = map;
-    back[warp][lane] = back_b;
-    if (lane == 0) {
-      cut[warp] = rows.starts;
-      cut_back[warp] = rows.ends;
+    for (int i = S - 1; i >= 0; --i) {
+      if (i < left) back.b = D::fade(kept[i], add(unpack<io_t>(dy[i * 32]), back.b));
     }
-    __syncthreads();
-    const Tile next = coming[(round + 1) & 1];
-    fetch(next, (round + 1) & 1);
-
-    // the map of the warps behind this one; the last warp joins all of them and publishes the tile's
-    const bool open = index > 0 && (cut_back[kWarps - 1] >> (S - 1) & 1) == 0;  // the last row's sequence goes on
-    const int group = index / kGroup, before = index % kGroup;
-    bool cut_behind = false;
-    Map<V> behind = Map<V>::identity();
-    const int stop = warp == kWarps - 1 ? 0 : warp + 1;
-    for (int w = kWarps - 1; w >= stop; --w) {
-      const Map<V> m{pieces[w][lane].a, back[w][lane]};
-      if (cut_back[w] != 0) {
-        behind = m;
-        cut_behind = true;
-      } else {
-        behind.then(m);
+    back.a = map.a;
+    const Map<V> behind = Scan<V>::join_groups(back);
+    if (lane >= 32 - kLanes) pieces[buffer][warp][lane % kLanes] = back;
+    // h before this lane's rows: lane groups are counted against time, so their maps come from the lanes above
+    L h = saved;
+#pragma unroll
+    for (int gr = kGroups - 1; gr > 0; --gr) {
+      Map<V> m;
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) {
+        const int from = gr * kLanes + lane % kLanes;
+        m.a.v[i] = make_float2(__shfl_sync(0xffffffffu, map.a.v[i].x, from), __shfl_sync(0xffffffffu, map.a.v[i].y, from));
+        m.b.v[i] = make_float2(__shfl_sync(0xffffffffu, map.b.v[i].x, from), __shfl_sync(0xffffffffu, map.b.v[i].y, from));
       }
+      if (lane / kLanes < gr) h = m.apply(h);
     }
-    const bool publish = index + 1 < chain.tiles;
-    if (warp == kWarps - 1 && publish) Chain<V>::publish(chain, tile.block, index, behind, cut_behind);
-    L c = L::all(0.0f);
     // what ddecay needs of the states: the state before every row, less its input (complement)
-    for (int w = 0; w < warp; ++w) {
-      const Map<V> m = pieces[w][lane];
-      h = cut[w] != 0 ? m.b : m.apply(h);
-    }
     L states[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      if (rows.starts >> i & 1) h = state_of(p.initial, i);
       const L value = unpack<io_t>(x[i * 32]);
       states[i] = COMPLEMENT ? minus(h, value) : h;
       h = D::step(kept[i], h, value);
     }
-    if (warp == kWarps - 1) {
-      if (open) c = Chain<V>::state_before(chain, tile.block, group, before);
-      carry[lane] = c;
-    }
+    fetch(next, buffer ^ 1);
     __syncthreads();
-    c = carry[lane];
-    if (warp == kWarps - 1) {
-      if (publish && before == kGroup - 1)
-        Chain<V>::put(Chain<V>::state_at(chain, tile.block, group), cut_behind ? behind.b : behind.apply(c));
-    } else {
-      c = cut_behind ? behind.b : behind.apply(c);
-    }
 
-    io_t* dx = static_cast<io_t*>(g.dx) + static_cast<long long>(row) * p.channels + channel;
-    io_t* dd = static_cast<io_t*>(g.ddecay) + static_cast<long long>(row) * p.channels + channel;
+    L c = carry;
+    if constexpr (CLUSTER) {
+      Map<V> cta = pieces[buffer][0][lane % kLanes];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w][lane % kLanes]);
+      c = join_cluster<V>(cta, slots[buffer], carry);
+      for (int w = 0; w < warp; ++w) c = pieces[buffer][w][lane % kLanes].apply(c);
+    } else {
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        if (w == warp) c = carry;
+        carry = pieces[buffer][w][lane % kLanes].apply(carry);
+      }
+    }
+    c = behind.apply(c);
+    if (next.seq != tile.seq) carry = final_grad(next);
+
+    // second sweep
+    const long long row = tile.begin + tile.at + own;
+    io_t* dx = static_cast<io_t*>(g.dx) + row * p.channels + channel;
+    io_t* dd = static_cast<io_t*>(g.ddecay) + row * p.channels + channel;
 #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-      const L grad = add(unpack<io_t>(dy[i * 32]), (rows.ends >> i & 1) ? state_of(g.dfinal, i) : c);
-      c = D::fade(kept[i], grad);
-      if (row + i < active) {
+      if (i < left) {
+        const L grad = add(unpack<io_t>(dy[i * 32]), c);
+        c = D::fade(kept[i], grad);
         A::store(dx + static_cast<long long>(i) * p.channels, D::input_grad(kept[i], grad), count);
         L drho = mul(grad, states[i]);
         if constexpr (LOGITS) drho = mul(drho, D::slope(D::sigmoid(unpack<io_t>(d[i * 32]), L::all(0.0f)), kept[i]));
         A::store(dd + static_cast<long long>(i) * p.channels, drho, count);
       }
-      if ((rows.starts >> i & 1) && g.dinitial != nullptr)
-        store_states<V>(g.dinitial + static_cast<long long>(rows.seq_of(i)) * p.channels + channel, c, count);
     }
+    if (tile.at + own == 0 && g.dinitial != nullptr)
+      store_states<V>(g.dinitial + static_cast<long long>(tile.seq) * p.channels + channel, c, count);
     tile = next;
   }
-  copies_done<0>();
 }
 
 // ---- launches
-
-// Where the chain lives in the workspace.  All of it is filled with kEmpty by every call that uses it.
-ChainSpace chain_space(void* workspace, int total, int channels, int lanes, long long* bytes) {
-  ChainSpace c{};
-  c.tiles = (total + kTile - 1) / kTile;
-  c.groups = (c.tiles + kGroup - 1) / kGroup;
-  c.blocks = (channels + lanes - 1) / lanes;
-  char* base = static_cast<char*>(workspace);
-  const long long maps = 8ll * c.tiles * c.blocks * lanes, states = 4ll * c.groups * c.blocks * lanes;
-  c.ticket = reinterpret_cast<int*>(base);
-  c.maps = reinterpret_cast<float*>(base + 256);
-  c.states = reinterpret_cast<float*>(base + 256 + maps);
-  *bytes = c.tiles > 1 ? 256 + maps + states : 0;
-  return c;
-}
 
 int sm_count() {
   static const int count = [] {
@@ -490,21 +472,16 @@ bool multiple_of(int bytes, std::initializer_list<const void*> pointers) {
   return true;
 }
 
-int check_sizes(const char* what, int n_seq, int total, int channels, int io_dtype, int decay_mode, int input_mode,
-                const void* workspace, size_t workspace_bytes) {
+int check_sizes(const char* what, int n_seq, int total, int channels, int io_dtype, int decay_mode, int input_mode) {
   if (n_seq <= 0 || n_seq > 65535) return fail(FRWKV_ERR_ARGUMENT, "%s: sequence count must be in 1..65535, got %d", what, n_seq);
   if (total < n_seq || channels <= 0)
     return fail(FRWKV_ERR_ARGUMENT, "%s: every sequence needs a token and there must be a channel", what);
-  if (static_cast<long long>((total + kTile - 1) / kTile) * ((channels + 31) / 32) > 0x7f000000ll)
-    return fail(FRWKV_ERR_UNSUPPORTED, "%s: more than 2^31 tiles of %d tokens by 32 channels", what, kTile);
+  if (channels > 0x7fffff00 || total > 0x7ffff000)
+    return fail(FRWKV_ERR_UNSUPPORTED, "%s: token and channel counts must leave room for a tile below 2^31", what);
   if (io_dtype < FRWKV_IO_BF16 || io_dtype > FRWKV_IO_FP32) return fail(FRWKV_ERR_UNSUPPORTED, "%s: unknown token dtype", what);
   if ((decay_mode != FRWKV_DECAY_LOGITS && decay_mode != FRWKV_DECAY_RETENTION) ||
       (input_mode != FRWKV_INPUT_UNIT && input_mode != FRWKV_INPUT_COMPLEMENT))
     return fail(FRWKV_ERR_ARGUMENT, "%s: unknown decay or input mode", what);
-  if (workspace_bytes < frwkv_sm100_gated_scan_workspace_bytes(total, channels) ||
-      (workspace == nullptr && workspace_bytes > 0) || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)
-    return fail(FRWKV_ERR_WORKSPACE, "%s: the workspace must be 16-byte aligned and hold %zu bytes", what,
-                frwkv_sm100_gated_scan_workspace_bytes(total, channels));
   return FRWKV_OK;
 }
 
@@ -541,28 +518,58 @@ int granule_of(const GatedScanParams& p, int io_dtype, std::initializer_list<con
   return element;
 }
 
-// Launches a chained kernel: fills the chain's space, as many CTAs as are resident at most.
+// How the work is cut.  Few sequences with few channels leave the GPU empty, so a cluster shares a sequence: the size that
+// needs the fewest rounds of CTAs for its work (`slots` CTAs are resident at a time), a smaller one where that gains less
+// than 5 % (a cluster's barrier costs a step about that).  Very many sequences are taken several to a unit, so that the
+// CTAs outlive their start.
+Grid cut(const GatedScanParams& p, int max_seqlen, int lanes, int slots) {
+  Grid g{(p.channels + lanes - 1) / lanes, 1, 1};
+  const long long items = static_cast<long long>(p.n_seq) * g.blocks;
+  g.per_unit = static_cast<int>(std::min<long long>(32, std::max<long long>(1, items / 16384)));
+  const long long units = static_cast<long long>((p.n_seq + g.per_unit - 1) / g.per_unit) * g.blocks;
+  const int longest = max_seqlen > 0 ? max_seqlen : (p.total + p.n_seq - 1) / p.n_seq;
+  const int tiles = (longest + kTile - 1) / kTile;
+  double best = 0.0;
+  for (int size = 1; size <= kMaxCluster && size <= tiles; ++size) {
+    const double time = static_cast<double>((units * size + slots - 1) / slots) * ((tiles + size - 1) / size);
+    if (size == 1 || time < 0.95 * best) {
+      best = time;
+      g.cluster = size;
+    }
+  }
+  return g;
+}
+
 template <typename K, typename... Args>
-int launch_chained(K kernel, int lanes, int threads, int tensors, int ctas, const GatedScanParams& p, void* workspace, cudaStream_t s,
-                   const char* what, Args... args) {
-  long long bytes;
-  const ChainSpace chain = chain_space(workspace, p.total, p.channels, lanes, &bytes);
-  const int shared = tensors * kTile * 256;  // 256-byte rows
-  cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
-  if (error == cudaSuccess && chain.tiles > 1) error = cudaMemsetAsync(workspace, 0xff, bytes, s);
+int launch(K kernel, const Grid& g, const GatedScanParams& p, int tensors, void* stream, const char* what, Args... args) {
+  const long long units = static_cast<long long>((p.n_seq + g.per_unit - 1) / g.per_unit) * g.blocks;
+  if (units * g.cluster > 0x7fffffffll) return fail(FRWKV_ERR_UNSUPPORTED, "%s: too many sequences by channels", what);
+  const int shared = 2 * tensors * kTile * kLanes * 8;  // two tiles
+  const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
   if (error != cudaSuccess) return fail(FRWKV_ERR_CUDA, "%s: preparing the launch: %s", what, cudaGetErrorString(error));
-  const long long tiles = static_cast<long long>(chain.tiles) * chain.blocks, resident = static_cast<long long>(ctas) * sm_count();
-  const unsigned grid = static_cast<unsigned>(chain.tiles > 1 && tiles > resident ? resident : tiles);
-  kernel<<<grid, threads, shared, s>>>(p, args..., chain);
+  cudaLaunchAttribute cluster;
+  cluster.id = cudaLaunchAttributeClusterDimension;
+  cluster.val.clusterDim.x = static_cast<unsigned>(g.cluster);
+  cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(units * g.cluster));
+  config.blockDim = dim3(kThreads);
+  config.dynamicSmemBytes = static_cast<size_t>(shared);
+  config.stream = static_cast<cudaStream_t>(stream);
+  config.attrs = &cluster;
+  config.numAttrs = g.cluster > 1 ? 1 : 0;
+  cudaLaunchKernelEx(&config, kernel, p, args..., g);
   return check_launch(what);
 }
 
-int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, void* workspace, void* stream) {
+int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream) {
   int rc = FRWKV_OK;
   with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
-      rc = launch_chained(gated_scan_forward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), kThreads + 32, 3 * 2,
-                          kForwardCtas, p, workspace, static_cast<cudaStream_t>(stream), "gated_scan_forward_kernel");
+      using io_t = decltype(io);
+      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kForwardCtas * sm_count());
+      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), true>, g, p, 2, stream, "gated_scan_forward_kernel")
+                         : launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), false>, g, p, 2, stream, "gated_scan_forward_kernel");
     });
   });
   return rc;
@@ -589,74 +596,71 @@ int run_steps(const GatedScanParams& p, int io_dtype, int decay_mode, int input_
 }  // namespace
 }  // namespace frwkv
 
-extern "C" size_t frwkv_sm100_gated_scan_workspace_bytes(int total_tokens, int channels) {
-  if (total_tokens <= 0 || channels <= 0) return 0;
-  long long wide, narrow;  // channel blocks of fp32 and of 16-bit tokens
-  frwkv::chain_space(nullptr, total_tokens, channels, 64, &wide);
-  frwkv::chain_space(nullptr, total_tokens, channels, 128, &narrow);
-  return static_cast<size_t>(wide > narrow ? wide : narrow);
-}
-
 extern "C" int frwkv_sm100_gated_scan(
     const int32_t* cu_seqlens, const int32_t* slots, const int32_t* status, float* state_pool, const void* x,
     long long x_row_stride, const void* decay, long long decay_row_stride, const void* decay_bias, void* y, int n_seq,
-    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* workspace,
-    size_t workspace_bytes, void* stream) {
+    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream) {
   using namespace frwkv;
   if (!cu_seqlens || !slots || !state_pool || !x || !decay || !y)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan: cu_seqlens, slots, state_pool, x, decay and y must be non-null");
   if (decay_bias != nullptr && decay_mode != FRWKV_DECAY_LOGITS)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan: decay_bias only applies to decay logits");
-  const int bad = check_sizes("gated_scan", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode, workspace,
-                              workspace_bytes);
+  const int bad = check_sizes("gated_scan", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode);
   if (bad != FRWKV_OK) return bad;
+  // short sequences go through the step kernel, the others through the tiled one; where it is known that there are none of
+  // one kind, its kernel is not launched.  (The step kernel counts its threads in 32 bits.)
+  const bool step_fits = static_cast<long long>(n_seq) * channels < 0x7fffffffll;
+  const bool all_short = step_fits && max_seqlen > 0 && max_seqlen <= kShortRows;
+  const bool none_short = !step_fits || n_seq == 1 || (max_seqlen > 0 && static_cast<long long>(max_seqlen) * n_seq == total_tokens);
   const GatedScanParams p{cu_seqlens, slots, status, x, decay, decay_bias, x_row_stride, decay_row_stride, state_pool,
-                          state_pool, nullptr, y, n_seq, total_tokens, channels, 0};
-  if (max_seqlen == 1 && static_cast<long long>(n_seq) * channels < 0x7fffffffll)
-    return run_steps(p, io_dtype, decay_mode, input_mode, stream);
-  return run_forward(p, io_dtype, decay_mode, input_mode, workspace, stream);
+                          state_pool, nullptr, y, n_seq, total_tokens, channels, 0,
+                          all_short ? 0x7fffffff : none_short ? 0 : kShortRows};
+  int rc = FRWKV_OK;
+  if (all_short || !none_short) rc = run_steps(p, io_dtype, decay_mode, input_mode, stream);
+  if (rc == FRWKV_OK && !all_short) rc = run_forward(p, io_dtype, decay_mode, input_mode, max_seqlen, stream);
+  return rc;
 }
 
 extern "C" int frwkv_sm100_gated_scan_train_forward(
     const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
     long long decay_row_stride, const float* initial, void* y, float* final_state, float* boundary, int n_seq,
-    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, void* workspace,
-    size_t workspace_bytes, void* stream) {
+    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream) {
   using namespace frwkv;
   if (!x || !decay || !y || !final_state || !boundary)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan training: x, decay, y, final_state and boundary must be non-null");
-  const int bad = check_sizes("gated_scan training", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode,
-                              workspace, workspace_bytes);
+  const int bad = check_sizes("gated_scan training", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode);
   if (bad != FRWKV_OK) return bad;
   if (cu_seqlens == nullptr && total_tokens % n_seq != 0)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan training: dense rows must be a multiple of the sequence count");
   const GatedScanParams p{cu_seqlens, nullptr, status, x, decay, nullptr, x_row_stride, decay_row_stride, initial,
-                          final_state, boundary, y, n_seq, total_tokens, channels, total_tokens / n_seq};
-  return run_forward(p, io_dtype, decay_mode, input_mode, workspace, stream);
+                          final_state, boundary, y, n_seq, total_tokens, channels, total_tokens / n_seq, 0};
+  return run_forward(p, io_dtype, decay_mode, input_mode, max_seqlen, stream);
 }
 
 extern "C" int frwkv_sm100_gated_scan_train_backward(
     const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
     long long decay_row_stride, const float* initial, const float* boundary, const void* dy, const float* dfinal,
     void* dx, void* ddecay, float* dinitial, int n_seq, int total_tokens, int channels, int io_dtype, int decay_mode,
-    int input_mode, void* workspace, size_t workspace_bytes, void* stream) {
+    int input_mode, int max_seqlen, void* stream) {
   using namespace frwkv;
   if (!x || !decay || !boundary || !dy || !dx || !ddecay)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan backward: x, decay, boundary, dy, dx and ddecay must be non-null");
-  const int bad = check_sizes("gated_scan backward", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode,
-                              workspace, workspace_bytes);
+  const int bad = check_sizes("gated_scan backward", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode);
   if (bad != FRWKV_OK) return bad;
   if (cu_seqlens == nullptr && total_tokens % n_seq != 0)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan backward: dense rows must be a multiple of the sequence count");
   const GatedScanParams p{cu_seqlens, nullptr, status, x, decay, nullptr, x_row_stride, decay_row_stride, initial,
                           nullptr, const_cast<float*>(boundary), nullptr, n_seq, total_tokens, channels,
-                          total_tokens / n_seq};
+                          total_tokens / n_seq, 0};
   const GatedScanGrads g{dy, dfinal, dx, ddecay, dinitial};
   int rc = FRWKV_OK;
   with_type(io_dtype, granule_of(p, io_dtype, {x, decay, dy, dx, ddecay}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
-      rc = launch_chained(gated_scan_backward_kernel<decltype(io), granule(), logits(), complement()>, 256 / static_cast<int>(sizeof(io)), kThreads, 2 * 3,
-                          kBackwardCtas, p, workspace, static_cast<cudaStream_t>(stream), "gated_scan_backward_kernel", g);
+      using io_t = decltype(io);
+      const Grid grid = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kBackwardCtas * sm_count());
+      rc = grid.cluster > 1
+               ? launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), true>, grid, p, 3, stream, "gated_scan_backward_kernel", g)
+               : launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), false>, grid, p, 3, stream, "gated_scan_backward_kernel", g);
     });
   });
   return rc;

@@ -1,4 +1,4 @@
-// Arithmetic, row metadata and the chain between tiles that the gated scan's kernels share.
+// Arithmetic and memory accesses that the gated scan's kernels share.
 //
 //   h_t = rho_t * h_{t-1} + i_t * x_t,   rho = exp(-s), s = exp(-1/2) * sigmoid(logit + bias)   or rho itself.
 // From logits the kernels work with rho - 1 and write rho * h as h + (rho - 1) * h: a slow channel has 1 - rho of 1e-4
@@ -20,10 +20,17 @@ struct GatedScanParams {
   long long x_stride, decay_stride;
   const float* initial;  // read at the first token of a sequence; null: zeros
   float* final_state;    // written behind the last token (the pool itself for the in-place operator)
-  float* boundary;       // training: the state before every FRWKV_GATED_SCAN_TILE-th row
+  float* boundary;       // training: the state before every kSavedRows-th row of a sequence, see saved_row()
   void* y;
   int n_seq, total, channels, seq_len;
+  int longer_than;  // sequences of at most this many tokens are left to the step kernel
 };
+
+constexpr int kSavedRows = FRWKV_GATED_SCAN_SAVED_ROWS;
+
+// Where the state before row `at` (a multiple of kSavedRows) of a sequence that begins at row `first` is saved: sequences
+// leave room for each other, and total / kSavedRows + n_seq rows hold all of them.
+__device__ __forceinline__ long long saved_row(int seq, int first, int at) { return first / kSavedRows + seq + at / kSavedRows; }
 
 struct GatedScanGrads {
   const void* dy;
@@ -207,76 +214,7 @@ template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
   }
 };
 
-// ---- rows and sequences
-
-// The sequences that S consecutive rows of a warp belong to.
-struct RowMap {
-  int seq;          // of the first row
-  unsigned starts;  // bit i: row i is the first of its sequence
-  unsigned ends;    // bit i: row i is the last of its sequence
-
-  // sequence of row i
-  __device__ __forceinline__ int seq_of(int i) const { return seq + __popc(starts & ((2u << i) - 2u)); }
-};
-
-// Rows [row, row + S) of `active`; all lanes of the warp take part.  S < 31.
-template <int S> __device__ __forceinline__ RowMap map_rows(const GatedScanParams& p, int row, int active, int n_seq) {
-  const int lane = threadIdx.x & 31;
-  RowMap m;
-  unsigned bounds;  // bit i: a sequence starts at row + i (or the last one ends before it)
-  if (p.cu == nullptr) {
-    m.seq = row / p.seq_len;
-    const int into = row - m.seq * p.seq_len;  // of the first row's sequence
-    if (p.seq_len > S) {  // at most one bound, behind the first row
-      bounds = (into == 0 ? 1u : 0u) | (p.seq_len - into <= S ? 1u << (p.seq_len - into) : 0u);
-    } else {
-      bounds = __ballot_sync(0xffffffffu, lane <= S && (into + lane) % p.seq_len == 0);
-    }
-  } else {
-    int low = 0, high = n_seq;  // cu[low] <= row < cu[high]
-    while (high - low > 1) {
-      const int step = (high - low + 31) / 32, at = low + lane * step;
-      const int below = __popc(__ballot_sync(0xffffffffu, at < high && p.cu[at] <= row));
-      low += (below - 1) * step;
-      high = min(low + step, high);
-    }
-    m.seq = low;
-    const int bound = low + lane <= n_seq ? p.cu[low + lane] : -1;
-    const bool inside = bound >= row && bound <= row + S;
-    bounds = __reduce_or_sync(0xffffffffu, inside ? 1u << (bound - row) : 0u);
-  }
-  const unsigned live = row + S <= active ? (1u << S) - 1 : row < active ? (1u << (active - row)) - 1 : 0u;
-  m.starts = bounds & live;
-  m.ends = (bounds >> 1) & live;
-  return m;
-}
-
-// ---- the chain between tiles
-//
-// A tile of rows turns the state h before it into A h + B (B alone behind a sequence's start).  Tiles publish (A, B) as
-// soon as they have them; the last tile of every kGroup also publishes the state behind it.  A tile joins the published
-// maps of the tiles before it in its group and applies them to the state behind the group before: one hop of the serial
-// chain covers kGroup tiles.  What is joined, and in which order, depends on the rows alone and never on timing.
-// Tiles are handed out in order by a counter, so what a tile waits for is always in work or done.
-//
-// Every published word says by itself whether it is there: the call first fills the space with kEmpty, no value is ever
-// stored with those bits (a NaN is stored as another one), and a reader takes a word once it differs.  So one trip to L2
-// brings flag and value together, and nothing has to be fenced.
-
-constexpr int kGroup = 16;
-constexpr unsigned kEmpty = 0xffffffffu;  // of the filled space
-constexpr unsigned kCut = 0x7fc0c0deu;    // A of a tile in which a sequence starts (backward: ends)
-constexpr int kSpinLimit = 1 << 20;       // about a second of polling; then the state becomes NaN and the kernel ends
-
-// Any value but kEmpty and kCut: a NaN other than the marks becomes the plain one.
-__device__ __forceinline__ float storable(float x) { return x == x ? x : __int_as_float(0x7fffffff); }
-
-struct ChainSpace {
-  int* ticket;    // kEmpty at first: the first ticket is 0 after adding 1 to what was there
-  float* maps;    // [blocks][tiles][A or B][lane][V]
-  float* states;  // [blocks][groups][lane][V]
-  int tiles, groups, blocks;  // time tiles, groups of them, channel blocks
-};
+// ---- affine maps h -> a h + b
 
 template <int V> struct alignas(4 * V) Map {
   Lanes<V> a, b;
@@ -290,84 +228,12 @@ template <int V> struct alignas(4 * V) Map {
   }
 };
 
-template <int V> struct Chain {
-  using L = Lanes<V>;
-
-  static __device__ __forceinline__ void put_raw(float* to, const L& x) {
-    if constexpr (V == 4)
-      asm volatile("st.relaxed.gpu.global.v4.f32 [%0], {%1, %2, %3, %4};"
-                   : : "l"(to), "f"(x.v[0].x), "f"(x.v[0].y), "f"(x.v[1].x), "f"(x.v[1].y) : "memory");
-    else
-      asm volatile("st.relaxed.gpu.global.v2.f32 [%0], {%1, %2};" : : "l"(to), "f"(x.v[0].x), "f"(x.v[0].y) : "memory");
-  }
-  static __device__ __forceinline__ void put(float* to, const L& x) { put_raw(to, each([](float v) { return storable(v); }, x)); }
-  static __device__ __forceinline__ L look(const float* from) {
-    L x;
-    if constexpr (V == 4)
-      asm volatile("ld.relaxed.gpu.global.v4.f32 {%0, %1, %2, %3}, [%4];"
-                   : "=f"(x.v[0].x), "=f"(x.v[0].y), "=f"(x.v[1].x), "=f"(x.v[1].y) : "l"(from) : "memory");
-    else
-      asm volatile("ld.relaxed.gpu.global.v2.f32 {%0, %1}, [%2];" : "=f"(x.v[0].x), "=f"(x.v[0].y) : "l"(from) : "memory");
-    return x;
-  }
-  static __device__ __forceinline__ bool there(const L& x) {
-    bool yes = true;
+template <int V> __device__ __forceinline__ Lanes<V> shuffle_up(const Lanes<V>& x, int lanes) {
+  Lanes<V> r;
 #pragma unroll
-    for (int i = 0; i < V / 2; ++i) yes = yes && __float_as_uint(x.v[i].x) != kEmpty && __float_as_uint(x.v[i].y) != kEmpty;
-    return yes;
-  }
-  static __device__ __forceinline__ L wait(const float* from, L x) {  // x: what an earlier look brought
-    for (int i = 0; i < kSpinLimit && !there(x); ++i) x = look(from);
-    return there(x) ? x : L::all(__int_as_float(0x7fffffff));
-  }
-  static __device__ __forceinline__ float* map_at(const ChainSpace& c, int block, int index) {
-    return c.maps + ((static_cast<long long>(block) * c.tiles + index) * 64 + (threadIdx.x & 31)) * V;
-  }
-  static __device__ __forceinline__ float* state_at(const ChainSpace& c, int block, int group) {
-    return c.states + ((static_cast<long long>(block) * c.groups + group) * 32 + (threadIdx.x & 31)) * V;
-  }
-  // One warp publishes its tile's map; index counts tiles in the chain's direction.
-  static __device__ __forceinline__ void publish(const ChainSpace& c, int block, int index, const Map<V>& m, bool cut) {
-    float* to = map_at(c, block, index);
-    if (cut) put_raw(to, L::all(__uint_as_float(kCut)));
-    else put(to, m.a);
-    put(to + 32 * V, m.b);
-  }
-  static __device__ __forceinline__ bool is_cut(const L& a) { return __float_as_uint(a.v[0].x) == kCut; }  // all lanes agree
-  // The state before a tile, by one warp: the maps of the n < kGroup tiles before it in its group behind the state that
-  // the group before left.  All maps are asked for in batches before the first is waited for.
-  static __device__ __forceinline__ L state_before(const ChainSpace& c, int block, int group, int n) {
-    L state = L::all(0.0f);
-    if (group > 0) state = look(state_at(c, block, group - 1));
-    Map<V> all = Map<V>::identity();
-    bool cut = false;
-    constexpr int kBatch = 8;
-    for (int base = 0; base < n; base += kBatch) {
-      const float* from = map_at(c, block, group * kGroup + base);
-      Map<V> m[kBatch];
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        const float* at = from + (base + i < n ? i : 0) * 64 * V;
-        m[i].a = look(at);
-        m[i].b = look(at + 32 * V);
-      }
-#pragma unroll
-      for (int i = 0; i < kBatch; ++i) {
-        if (base + i >= n) break;
-        m[i].a = wait(from + i * 64 * V, m[i].a);
-        m[i].b = wait(from + i * 64 * V + 32 * V, m[i].b);
-        if (is_cut(m[i].a)) {
-          all.b = m[i].b;
-          cut = true;
-        } else {
-          all.then(m[i]);
-        }
-      }
-    }
-    if (cut) return all.b;
-    if (group == 0) return L::all(__int_as_float(0x7fffffff));  // no sequence starts at row 0: not valid
-    return all.apply(wait(state_at(c, block, group - 1), state));
-  }
-};
+  for (int i = 0; i < V / 2; ++i)
+    r.v[i] = make_float2(__shfl_up_sync(0xffffffffu, x.v[i].x, lanes), __shfl_up_sync(0xffffffffu, x.v[i].y, lanes));
+  return r;
+}
 
 }  // namespace frwkv

@@ -249,33 +249,29 @@ int frwkv_sm100_wkv7_pretrain_backward(const void* r, const void* w, const void*
  *   y          : [total_tokens, channels], contiguous, token dtype;
  *   cu_seqlens, slots, status, max_seqlen : as in frwkv_sm100_wkv7_recurrent, with the same fail-closed rules
  *                (invalid metadata: y NaN-filled, pool untouched; rows behind the last active sequence untouched);
- *   workspace  : device scratch of frwkv_sm100_gated_scan_workspace_bytes(total_tokens, channels) bytes, 16-byte
- *                aligned, for this call alone until it has finished (two calls that may overlap need two).
- * Any number of channels; channels and strides that are multiples of 8 (16-byte rows) run fastest. */
-size_t frwkv_sm100_gated_scan_workspace_bytes(int total_tokens, int channels);
+ * Any number of channels; channels, strides and starts that are multiples of 8 bytes run fastest. */
 int frwkv_sm100_gated_scan(
     const int32_t* cu_seqlens, const int32_t* slots, const int32_t* status, float* state_pool, const void* x,
     long long x_row_stride, const void* decay, long long decay_row_stride, const void* decay_bias, void* y, int n_seq,
-    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* workspace,
-    size_t workspace_bytes, void* stream);
+    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream);
 
 /* The gated scan as a training operator.  Rows are n_seq sequences of total_tokens / n_seq tokens each (cu_seqlens
  * NULL), or packed by cu_seqlens [n_seq+1], whose status word then rules as above (invalid: outputs NaN-filled).
  *   initial  : fp32 [n_seq, channels] or NULL (zeros);   final_state : fp32 [n_seq, channels];
- *   boundary : fp32 [ceil(total_tokens / FRWKV_GATED_SCAN_TILE), channels], saved for the backward pass: the state
- *              before the first token of every tile of rows;
+ *   boundary : fp32 [total_tokens / FRWKV_GATED_SCAN_SAVED_ROWS + n_seq, channels], saved for the backward pass: the
+ *              state before every FRWKV_GATED_SCAN_SAVED_ROWS-th token of every sequence;
+ *   max_seqlen : largest sequence length of packed rows (a launch-shape hint; <= 0 if unknown);
  *   dy, dx, ddecay : contiguous, token dtype;  dfinal (NULL: zeros), dinitial (NULL: not wanted) : fp32. */
-#define FRWKV_GATED_SCAN_TILE 64
+#define FRWKV_GATED_SCAN_SAVED_ROWS 32
 int frwkv_sm100_gated_scan_train_forward(
     const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
     long long decay_row_stride, const float* initial, void* y, float* final_state, float* boundary, int n_seq,
-    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, void* workspace,
-    size_t workspace_bytes, void* stream);
+    int total_tokens, int channels, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream);
 int frwkv_sm100_gated_scan_train_backward(
     const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
     long long decay_row_stride, const float* initial, const float* boundary, const void* dy, const float* dfinal,
     void* dx, void* ddecay, float* dinitial, int n_seq, int total_tokens, int channels, int io_dtype, int decay_mode,
-    int input_mode, void* workspace, size_t workspace_bytes, void* stream);
+    int input_mode, int max_seqlen, void* stream);
 
 /* Log probabilities of given tokens under rows of vocabulary logits, with the entropy of each row and its most
  * probable tokens; forward and gradient.  No counterpart in the reference.  z = logits / temperature,

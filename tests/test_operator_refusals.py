@@ -126,19 +126,17 @@ def test_c_entries_refuse_bad_arguments():
     from flashrwkv2_b200 import _lib
 
     lib = _lib.load()
-    need = lib.frwkv_sm100_gated_scan_workspace_bytes(100, 64)
 
-    def scan(pool=16, n_seq=1, total=100, channels=64, io=0, decay=0, gate=0, bias=0, work=16, size=need):
-        return lib.frwkv_sm100_gated_scan(16, 16, 16, pool, 16, 64, 16, 64, bias, 16, n_seq, total, channels, io, decay, gate, 0,
-                                          work, size, 0)
+    def scan(pool=16, n_seq=1, total=100, channels=64, io=0, decay=0, gate=0, bias=0):
+        return lib.frwkv_sm100_gated_scan(16, 16, 16, pool, 16, 64, 16, 64, bias, 16, n_seq, total, channels, io, decay, gate, 0, 0)
 
     for bad, text in ((dict(pool=0), "non-null"), (dict(n_seq=0), "1..65535"), (dict(n_seq=65536, total=70000), "1..65535"),
-                      (dict(total=0), "token"), (dict(channels=0), "channel"), (dict(io=3), "dtype"), (dict(decay=2), "mode"),
+                      (dict(total=0), "token"), (dict(channels=0), "channel"), (dict(total=0x7fffffff), "2^31"), (dict(io=3), "dtype"), (dict(decay=2), "mode"),
                       (dict(gate=-1), "mode"), (dict(bias=16, decay=1), "decay_bias")):
         assert scan(**bad) != 0 and text in _lib.last_error(), bad
-    assert lib.frwkv_sm100_gated_scan_train_forward(0, 0, 16, 64, 16, 64, 0, 16, 16, 16, 3, 100, 64, 0, 0, 0, 16, need, 0) != 0
+    assert lib.frwkv_sm100_gated_scan_train_forward(0, 0, 16, 64, 16, 64, 0, 16, 16, 16, 3, 100, 64, 0, 0, 0, 0, 0) != 0
     assert "multiple of the sequence count" in _lib.last_error()
-    assert lib.frwkv_sm100_gated_scan_train_backward(0, 0, 16, 64, 16, 64, 0, 0, 16, 0, 16, 16, 0, 1, 100, 64, 0, 0, 0, 16, need, 0) != 0
+    assert lib.frwkv_sm100_gated_scan_train_backward(0, 0, 16, 64, 16, 64, 0, 0, 16, 0, 16, 16, 0, 1, 100, 64, 0, 0, 0, 0, 0) != 0
     assert "non-null" in _lib.last_error()
 
     def rows(outer=1, inner=1, vocab=8, io=0, temperature=1.0, k=0, ids=16):
