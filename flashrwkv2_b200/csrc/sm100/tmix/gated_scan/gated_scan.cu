@@ -18,13 +18,16 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int S = 8, kWarps = 8, kThreads = kWarps * 32;
-constexpr int kLanes = 8, kGroups = 32 / kLanes;  // lanes along the channels, groups of them along time
-constexpr int kWarpRows = kGroups * S, kTile = kWarps * kWarpRows;
-constexpr int kForwardCtas = 3, kBackwardCtas = 2;  // per SM: 64 KB and 96 KB of staging each
+constexpr int kTile = 256;           // tokens of a CTA's tile
+constexpr int kForwardRows = 16, kBackwardRows = 8;  // tokens of a lane in a tile
+constexpr int kForwardWarps = kTile / (kGroups * kForwardRows), kBackwardWarps = kTile / (kGroups * kBackwardRows);
+// CTAs per SM.  Copies of 4 bytes go through L1, which the staging of a fourth CTA would leave too small for rows that lie
+// across its lines (16 x 1024 rows of 1003 fp32 channels: 86 us with four, 56 us with three).
+constexpr int forward_ctas(int granule) { return granule == 16 ? 4 : 3; }
+constexpr int kBackwardCtas = 2;
 constexpr int kMaxCluster = 8;
-constexpr int kShortRows = 16;  // sequences of at most this many tokens are served by the step kernel
-static_assert(kWarpRows == kSavedRows, "the backward pass loads a state for every warp");
+constexpr int kShortRows = 16;       // sequences of at most this many tokens are served by the step kernel
+static_assert(kGroups * kBackwardRows == kSavedRows, "the backward pass loads a state for every warp");
 
 // NaN in every row that the call would write (fail-closed), by the whole grid.
 template <typename io_t>
@@ -74,7 +77,7 @@ template <int V> __device__ __forceinline__ Unit unit_of(const GatedScanParams& 
   return u;
 }
 
-// A CTA's tile: rows [row, row + kTile) of a sequence, which has `left` rows from there on (none, behind its end).
+// A CTA's tile: rows [at, at + kTile) of a sequence, as far as it goes.
 struct Tile {
   int seq;    // < 0: there is none
   int begin;  // first row of the sequence
@@ -108,7 +111,8 @@ __device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Map<V> (*slo
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  if (warp < ranks && lane < kLanes) cluster.map_shared_rank(&slots[rank][0], warp)[lane] = cta;
+  for (int r = warp; r < ranks; r += static_cast<int>(blockDim.x) / 32)
+    if (lane < kLanes) cluster.map_shared_rank(&slots[rank][0], r)[lane] = cta;
   cluster.sync();
   Lanes<V> mine = carry;
   for (int r = 0; r < ranks; ++r) {
@@ -121,13 +125,12 @@ __device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Map<V> (*slo
 // ---- forward
 
 template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
-  constexpr int V = 8 / sizeof(io_t);
+__global__ void __launch_bounds__(kForwardWarps * 32, forward_ctas(GRANULE)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
+  constexpr int V = 8 / sizeof(io_t), S = kForwardRows, kWarps = kForwardWarps;
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
-  using A = Access<io_t, GRANULE>;
-  extern __shared__ uint2 staged[];  // [2 tiles][x or decay][warp][S][lane]
-  constexpr int kTensor = kWarps * S * 32, kTileSpace = 2 * kTensor;
+  using R = Rows<io_t, GRANULE, S>;
+  extern __shared__ uint2 staged[];  // x of two tiles, then the decays of one: [warp][R::kWords]
   __shared__ Map<V> pieces[2][kWarps][kLanes], slots[2][CLUSTER ? kMaxCluster : 1][kLanes];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
@@ -139,6 +142,7 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_ker
   const int ranks = CLUSTER ? grid.cluster : 1, rank = CLUSTER ? static_cast<int>(blockIdx.x) % ranks : 0;
   Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, n_seq);
   const int channel = unit.channel, count = min(V, p.channels - channel);
+  const int block_channel = channel - lane % kLanes * V, block_count = min(kLanes * V, p.channels - block_channel);
   const auto first_tile = [&](int seq) {
     if (seq < 0) return Tile{-1, 0, 0, 0};
     const int begin = row_begin(p, seq);
@@ -148,19 +152,21 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_ker
     const int at = t.at + ranks * kTile;
     return at - rank * kTile < t.len ? Tile{t.seq, t.begin, at, t.len} : first_tile(unit.next());
   };
-  const int own = warp * kWarpRows + lane / kLanes * S;  // this lane's first row in a tile
+  const auto is_full = [&](const Tile& t) { return t.at + kTile <= t.len && block_count == kLanes * V; };
+  const int warp_row = warp * kGroups * S, own = warp_row + lane / kLanes * S;  // first rows in a tile
+  uint2* const decays = staged + (2 * kWarps + warp) * R::kWords;
+  const auto inputs = [&](int buffer) { return staged + (buffer * kWarps + warp) * R::kWords; };
   const auto fetch = [&](const Tile& t, int buffer) {
-    if (t.seq >= 0) {
-      const int left = t.len - t.at - own, row = t.begin + t.at + own;
-      const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
-      const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
-      uint2* to = staged + buffer * kTileSpace + warp * S * 32 + lane;
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const int n = i < left ? count : 0;
-        A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
-        A::stage(to + kTensor + i * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
-      }
+    if (t.seq < 0) return;
+    const int row = t.begin + t.at + warp_row, left = t.len - t.at - warp_row;
+    const io_t *x = static_cast<const io_t*>(p.x), *d = static_cast<const io_t*>(p.decay);
+    const io_t *x_rows = x + row * p.x_stride + block_channel, *d_rows = d + row * p.decay_stride + block_channel;
+    if (is_full(t)) {
+      R::template fetch<true>(inputs(buffer), x_rows, p.x_stride, left, block_count, x);
+      R::template fetch<true>(decays, d_rows, p.decay_stride, left, block_count, d);
+    } else {
+      R::template fetch<false>(inputs(buffer), x_rows, p.x_stride, left, block_count, x);
+      R::template fetch<false>(decays, d_rows, p.decay_stride, left, block_count, d);
     }
     copies_begun();
   };
@@ -186,17 +192,19 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_ker
     const int buffer = round & 1;
     const Tile next = tile_after(tile);
     copies_done();
-    const uint2* x = staged + buffer * kTileSpace + warp * S * 32 + lane;
+    __syncwarp();  // what the warp's other lanes copied
 
     // first sweep: the gates into registers, and the map of this lane's rows
+    const typename R::Mine x = R::mine(inputs(buffer), lane / kLanes), d = R::mine(decays, lane / kLanes);
     L kept[S];
     Map<V> map = Map<V>::identity();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      kept[i] = D::keep(unpack<io_t>(x[kTensor + i * 32]), bias);
-      map.b = D::step(kept[i], map.b, unpack<io_t>(x[i * 32]));
+      kept[i] = D::keep(d[i], bias);
+      map.b = D::step(kept[i], map.b, x[i]);
       map.a = D::fade(kept[i], map.a);
     }
+    __syncwarp();  // the decays have been read: their place is free
     fetch(next, buffer ^ 1);  // in flight while this tile is joined and written
     const Map<V> before = Scan<V>::join_groups(map);
     if (lane >= 32 - kLanes) pieces[buffer][warp][lane % kLanes] = map;
@@ -217,20 +225,32 @@ __global__ void __launch_bounds__(kThreads, kForwardCtas) gated_scan_forward_ker
         carry = pieces[buffer][w][lane % kLanes].apply(carry);
       }
     }
-    const int left = tile.len - tile.at - own;
-    if (p.boundary != nullptr && lane < kLanes && left > 0)
-      store_states<V>(p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel, h, count);
     h = before.apply(h);
+    const int left = tile.len - tile.at - own;
+    if (p.boundary != nullptr && own % kSavedRows == 0 && left > 0)
+      store_states<V>(p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel, h, count);
     if (next.seq != tile.seq) carry = initial_state(next);
 
     // second sweep
     io_t* y = static_cast<io_t*>(p.y) + static_cast<long long>(tile.begin + tile.at + own) * p.channels + channel;
+    if (is_full(tile)) {
 #pragma unroll
-    for (int i = 0; i < S; ++i) {
-      h = D::step(kept[i], h, unpack<io_t>(x[i * 32]));
-      if (i < left) A::store(y + static_cast<long long>(i) * p.channels, h, count);
-      if (i + 1 == left) store_states<V>(p.final_state + state_row(tile.seq), h, count);
+      for (int i = 0; i < S; ++i) {
+        h = D::step(kept[i], h, x[i]);
+        R::template store<true>(y, h, count);
+        y += p.channels;
+      }
+      if (left == S) store_states<V>(p.final_state + state_row(tile.seq), h, count);
+    } else {
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        h = D::step(kept[i], h, x[i]);
+        if (i < left) R::template store<false>(y, h, count);
+        if (i + 1 == left) store_states<V>(p.final_state + state_row(tile.seq), h, count);
+        y += p.channels;
+      }
     }
+    __syncwarp();  // the inputs have been read
     tile = next;
   }
 }
@@ -309,14 +329,13 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
 // pass.  The states come from those that the forward pass saved before every warp's rows.
 
 template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, kBackwardCtas)
+__global__ void __launch_bounds__(kBackwardWarps * 32, kBackwardCtas)
 gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const Grid grid) {
-  constexpr int V = 8 / sizeof(io_t);
+  constexpr int V = 8 / sizeof(io_t), S = kBackwardRows, kWarps = kBackwardWarps, kWarpRows = kGroups * S;
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
-  using A = Access<io_t, GRANULE>;
-  extern __shared__ uint2 staged[];  // [2 tiles][x, decay or dy][warp][S][lane]
-  constexpr int kTensor = kWarps * S * 32, kTileSpace = 3 * kTensor;
+  using R = Rows<io_t, GRANULE, S>;
+  extern __shared__ uint2 staged[];  // [2 tiles][x, decay or dy][warp][R::kWords]
   __shared__ Map<V> pieces[2][kWarps][kLanes], slots[2][CLUSTER ? kMaxCluster : 1][kLanes];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
@@ -327,6 +346,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   const int ranks = CLUSTER ? grid.cluster : 1, rank = CLUSTER ? static_cast<int>(blockIdx.x) % ranks : 0;
   Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, p.n_seq);
   const int channel = unit.channel, count = min(V, p.channels - channel);
+  const int block_channel = channel - lane % kLanes * V, block_count = min(kLanes * V, p.channels - block_channel);
   const int step_rows = ranks * kTile;
   const auto first_tile = [&](int seq) {
     if (seq < 0) return Tile{-1, 0, 0, 0};
@@ -336,21 +356,25 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   const auto tile_after = [&](const Tile& t) {
     return t.at >= step_rows ? Tile{t.seq, t.begin, t.at - step_rows, t.len} : first_tile(unit.next());
   };
-  const int own = (kWarps - 1 - warp) * kWarpRows + (kGroups - 1 - lane / kLanes) * S;
+  const auto is_full = [&](const Tile& t) { return t.at + kTile <= t.len && block_count == kLanes * V; };
+  // In memory the lane groups of a warp lie as in the forward pass, first in time first; along the chain a lane works on
+  // group kGroups - 1 - lane / kLanes.
+  const int warp_row = (kWarps - 1 - warp) * kWarpRows, group = kGroups - 1 - lane / kLanes, own = warp_row + group * S;
+  const auto space = [&](int buffer, int tensor) { return staged + ((buffer * 3 + tensor) * kWarps + warp) * R::kWords; };
   const auto fetch = [&](const Tile& t, int buffer) {
-    if (t.seq >= 0) {
-      const int left = t.len - t.at - own, row = t.begin + t.at + own;
-      const io_t* x = static_cast<const io_t*>(p.x) + row * p.x_stride + channel;
-      const io_t* d = static_cast<const io_t*>(p.decay) + row * p.decay_stride + channel;
-      const io_t* dy = static_cast<const io_t*>(g.dy) + static_cast<long long>(row) * p.channels + channel;
-      uint2* to = staged + buffer * kTileSpace + warp * S * 32 + lane;
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const int n = i < left ? count : 0;
-        A::stage(to + i * 32, n > 0 ? x + i * p.x_stride : static_cast<const io_t*>(p.x), n);
-        A::stage(to + kTensor + i * 32, n > 0 ? d + i * p.decay_stride : static_cast<const io_t*>(p.decay), n);
-        A::stage(to + 2 * kTensor + i * 32, n > 0 ? dy + static_cast<long long>(i) * p.channels : static_cast<const io_t*>(g.dy), n);
-      }
+    if (t.seq < 0) return;
+    const int row = t.begin + t.at + warp_row, left = t.len - t.at - warp_row;
+    const io_t *x = static_cast<const io_t*>(p.x), *d = static_cast<const io_t*>(p.decay), *dy = static_cast<const io_t*>(g.dy);
+    const io_t *x_rows = x + row * p.x_stride + block_channel, *d_rows = d + row * p.decay_stride + block_channel;
+    const io_t* dy_rows = dy + static_cast<long long>(row) * p.channels + block_channel;
+    if (is_full(t)) {
+      R::template fetch<true>(space(buffer, 0), x_rows, p.x_stride, left, block_count, x);
+      R::template fetch<true>(space(buffer, 1), d_rows, p.decay_stride, left, block_count, d);
+      R::template fetch<true>(space(buffer, 2), dy_rows, p.channels, left, block_count, dy);
+    } else {
+      R::template fetch<false>(space(buffer, 0), x_rows, p.x_stride, left, block_count, x);
+      R::template fetch<false>(space(buffer, 1), d_rows, p.decay_stride, left, block_count, d);
+      R::template fetch<false>(space(buffer, 2), dy_rows, p.channels, left, block_count, dy);
     }
     copies_begun();
   };
@@ -365,14 +389,14 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     const int buffer = round & 1, left = tile.len - tile.at - own;
     const Tile next = tile_after(tile);
     // the state before this warp's rows, where it has any
-    const int warp_at = tile.at + (kWarps - 1 - warp) * kWarpRows;
+    const int warp_at = tile.at + warp_row;
     const L saved = warp_at < tile.len
                         ? load_states<V>(p.boundary + saved_row(tile.seq, tile.begin, warp_at) * p.channels + channel, count)
                         : L::all(0.0f);
     copies_done();
-    const uint2* x = staged + buffer * kTileSpace + warp * S * 32 + lane;
-    const uint2* d = x + kTensor;
-    const uint2* dy = d + kTensor;
+    __syncwarp();  // what the warp's other lanes copied
+    const typename R::Mine x = R::mine(space(buffer, 0), group), d = R::mine(space(buffer, 1), group),
+                           dy = R::mine(space(buffer, 2), group);
 
     // first sweep: the gates, and the maps of h (rows in time) and c (against it).  Rows behind the sequence's end leave c as
     // it is.
@@ -380,13 +404,13 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     Map<V> map = Map<V>::identity(), back = map;
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      kept[i] = D::keep(unpack<io_t>(d[i * 32]), L::all(0.0f));
-      map.b = D::step(kept[i], map.b, unpack<io_t>(x[i * 32]));
+      kept[i] = D::keep(d[i], L::all(0.0f));
+      map.b = D::step(kept[i], map.b, x[i]);
       if (i < left) map.a = D::fade(kept[i], map.a);
     }
 #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-      if (i < left) back.b = D::fade(kept[i], add(unpack<io_t>(dy[i * 32]), back.b));
+      if (i < left) back.b = D::fade(kept[i], add(dy[i], back.b));
     }
     back.a = map.a;
     const Map<V> behind = Scan<V>::join_groups(back);
@@ -408,7 +432,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     L states[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      const L value = unpack<io_t>(x[i * 32]);
+      const L value = x[i];
       states[i] = COMPLEMENT ? minus(h, value) : h;
       h = D::step(kept[i], h, value);
     }
@@ -434,19 +458,26 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
 
     // second sweep
     const long long row = tile.begin + tile.at + own;
-    io_t* dx = static_cast<io_t*>(g.dx) + row * p.channels + channel;
-    io_t* dd = static_cast<io_t*>(g.ddecay) + row * p.channels + channel;
+    io_t* dx = static_cast<io_t*>(g.dx) + (row + S - 1) * p.channels + channel;
+    io_t* dd = static_cast<io_t*>(g.ddecay) + (row + S - 1) * p.channels + channel;
+    const auto sweep = [&](auto full) {
 #pragma unroll
-    for (int i = S - 1; i >= 0; --i) {
-      if (i < left) {
-        const L grad = add(unpack<io_t>(dy[i * 32]), c);
-        c = D::fade(kept[i], grad);
-        A::store(dx + static_cast<long long>(i) * p.channels, D::input_grad(kept[i], grad), count);
-        L drho = mul(grad, states[i]);
-        if constexpr (LOGITS) drho = mul(drho, D::slope(D::sigmoid(unpack<io_t>(d[i * 32]), L::all(0.0f)), kept[i]));
-        A::store(dd + static_cast<long long>(i) * p.channels, drho, count);
+      for (int i = S - 1; i >= 0; --i) {
+        if (full() || i < left) {
+          const L grad = add(dy[i], c);
+          c = D::fade(kept[i], grad);
+          R::template store<full()>(dx, D::input_grad(kept[i], grad), count);
+          L drho = mul(grad, states[i]);
+          if constexpr (LOGITS) drho = mul(drho, D::slope(D::sigmoid(d[i], L::all(0.0f)), kept[i]));
+          R::template store<full()>(dd, drho, count);
+        }
+        dx -= p.channels;
+        dd -= p.channels;
       }
-    }
+    };
+    if (is_full(tile)) sweep(std::true_type{});
+    else sweep(std::false_type{});
+    __syncwarp();  // everything has been read: the place is free
     if (tile.at + own == 0 && g.dinitial != nullptr)
       store_states<V>(g.dinitial + static_cast<long long>(tile.seq) * p.channels + channel, c, count);
     tile = next;
@@ -502,26 +533,28 @@ template <typename F> void with_modes(int decay_mode, int input_mode, F f) {
 template <typename F> void with_type(int io_dtype, int granule, F f) {
   using two = std::integral_constant<int, 2>;
   using four = std::integral_constant<int, 4>;
-  using eight = std::integral_constant<int, 8>;
-  if (io_dtype == FRWKV_IO_FP32) granule == 8 ? f(float{}, eight{}) : f(float{}, four{});
-  else if (io_dtype == FRWKV_IO_BF16) granule == 8 ? f(__nv_bfloat16{}, eight{}) : granule == 4 ? f(__nv_bfloat16{}, four{}) : f(__nv_bfloat16{}, two{});
-  else granule == 8 ? f(__half{}, eight{}) : granule == 4 ? f(__half{}, four{}) : f(__half{}, two{});
+  using all = std::integral_constant<int, 16>;
+  if (io_dtype == FRWKV_IO_FP32) granule == 16 ? f(float{}, all{}) : f(float{}, four{});
+  else if (io_dtype == FRWKV_IO_BF16) granule == 16 ? f(__nv_bfloat16{}, all{}) : granule == 4 ? f(__nv_bfloat16{}, four{}) : f(__nv_bfloat16{}, two{});
+  else granule == 16 ? f(__half{}, all{}) : granule == 4 ? f(__half{}, four{}) : f(__half{}, two{});
 }
 
-// The bytes of a token row that one access may move: 8 where the channels, the strides and all starts allow it.
+// The bytes of a token row that one access may move: 16 where the channels, the strides and all starts allow it, else 4, or
+// a 16-bit element.
 int granule_of(const GatedScanParams& p, int io_dtype, std::initializer_list<const void*> rows) {
   const int element = io_dtype == FRWKV_IO_FP32 ? 4 : 2;
-  for (int granule = 8; granule > element; granule /= 2) {
+  for (int granule : {16, 4}) {
     const int n = granule / element;
     if (p.channels % n == 0 && p.x_stride % n == 0 && p.decay_stride % n == 0 && multiple_of(granule, rows)) return granule;
   }
-  return element;
+  return 2;
 }
 
 // How the work is cut.  Few sequences with few channels leave the GPU empty, so a cluster shares a sequence: the size that
-// needs the fewest rounds of CTAs for its work (`slots` CTAs are resident at a time), a smaller one where that gains less
-// than 5 % (a cluster's barrier costs a step about that).  Very many sequences are taken several to a unit, so that the
-// CTAs outlive their start.
+// needs the least time in rounds of CTAs (`slots` are resident at once) times steps, a cluster's step counting half as much
+// again.  (65536 rows of 2048 channels: 462 us for single CTAs, 259 for four, 207 for eight; 8 x 4096 rows, where 512 single
+// CTAs fill the GPU: 80 us, and 92, 100, 116 us for clusters of 2, 4, 8.)  Very many sequences are taken several to a
+// unit, so that the CTAs outlive their start.
 Grid cut(const GatedScanParams& p, int max_seqlen, int lanes, int slots) {
   Grid g{(p.channels + lanes - 1) / lanes, 1, 1};
   const long long items = static_cast<long long>(p.n_seq) * g.blocks;
@@ -531,7 +564,7 @@ Grid cut(const GatedScanParams& p, int max_seqlen, int lanes, int slots) {
   const int tiles = (longest + kTile - 1) / kTile;
   double best = 0.0;
   for (int size = 1; size <= kMaxCluster && size <= tiles; ++size) {
-    const double time = static_cast<double>((units * size + slots - 1) / slots) * ((tiles + size - 1) / size);
+    const double time = static_cast<double>((units * size + slots - 1) / slots) * ((tiles + size - 1) / size) * (size > 1 ? 1.5 : 1.0);
     if (size == 1 || time < 0.95 * best) {
       best = time;
       g.cluster = size;
@@ -541,10 +574,10 @@ Grid cut(const GatedScanParams& p, int max_seqlen, int lanes, int slots) {
 }
 
 template <typename K, typename... Args>
-int launch(K kernel, const Grid& g, const GatedScanParams& p, int tensors, void* stream, const char* what, Args... args) {
+int launch(K kernel, const Grid& g, const GatedScanParams& p, int warps, int words, void* stream, const char* what, Args... args) {
   const long long units = static_cast<long long>((p.n_seq + g.per_unit - 1) / g.per_unit) * g.blocks;
   if (units * g.cluster > 0x7fffffffll) return fail(FRWKV_ERR_UNSUPPORTED, "%s: too many sequences by channels", what);
-  const int shared = 2 * tensors * kTile * kLanes * 8;  // two tiles
+  const int shared = warps * words * 8;
   const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
   if (error != cudaSuccess) return fail(FRWKV_ERR_CUDA, "%s: preparing the launch: %s", what, cudaGetErrorString(error));
   cudaLaunchAttribute cluster;
@@ -553,7 +586,7 @@ int launch(K kernel, const Grid& g, const GatedScanParams& p, int tensors, void*
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(units * g.cluster));
-  config.blockDim = dim3(kThreads);
+  config.blockDim = dim3(static_cast<unsigned>(warps) * 32);
   config.dynamicSmemBytes = static_cast<size_t>(shared);
   config.stream = static_cast<cudaStream_t>(stream);
   config.attrs = &cluster;
@@ -567,9 +600,11 @@ int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int inpu
   with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
-      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kForwardCtas * sm_count());
-      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), true>, g, p, 2, stream, "gated_scan_forward_kernel")
-                         : launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), false>, g, p, 2, stream, "gated_scan_forward_kernel");
+      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(granule()) * sm_count());
+      constexpr int kWords = 3 * Rows<io_t, granule(), kForwardRows>::kWords;
+      constexpr const char* kName = "gated_scan_forward_kernel";
+      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), true>, g, p, kForwardWarps, kWords, stream, kName)
+                         : launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), false>, g, p, kForwardWarps, kWords, stream, kName);
     });
   });
   return rc;
@@ -658,9 +693,10 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
       const Grid grid = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kBackwardCtas * sm_count());
-      rc = grid.cluster > 1
-               ? launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), true>, grid, p, 3, stream, "gated_scan_backward_kernel", g)
-               : launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), false>, grid, p, 3, stream, "gated_scan_backward_kernel", g);
+      constexpr int kWords = 6 * Rows<io_t, granule(), kBackwardRows>::kWords;
+      constexpr const char* kName = "gated_scan_backward_kernel";
+      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), true>, grid, p, kBackwardWarps, kWords, stream, kName, g)
+                            : launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), false>, grid, p, kBackwardWarps, kWords, stream, kName, g);
     });
   });
   return rc;

@@ -107,41 +107,86 @@ template <typename io_t> __device__ __forceinline__ uint2 pack(const Lanes<8 / s
   else return make_uint2(pack_pair<io_t>(a.v[0]), pack_pair<io_t>(a.v[1]));
 }
 
-// How much of a lane's 8 bytes one access may move: 8, 4 or (16-bit types at any alignment) 2 bytes.  `count` is how many
-// of the lane's elements exist.
-template <typename io_t, int GRANULE> struct Access {
-  static constexpr int V = 8 / sizeof(io_t), kElements = GRANULE / sizeof(io_t);
+// ---- token rows in shared memory
+//
+// A warp's rows of one tensor: four lane groups of S rows of 64 bytes each.  Odd groups have their rows swapped in pairs, so that
+// two groups that read their i-th rows at once read different banks.  GRANULE is how many bytes one access to global memory may move: 16, 8, 4 or, for 16-bit types
+// at any alignment, 2.  Copies are asynchronous but for 2 bytes, which the hardware cannot do; what does not exist becomes 0.
 
-  // One token's 8 bytes into shared memory, asynchronously where the hardware can (4 and 8 bytes), zeros for what does
-  // not exist.  A lane reads back only what it copied itself.
-  static __device__ __forceinline__ void stage(uint2* to, const io_t* from, int count) {
+constexpr int kLanes = 8, kGroups = 32 / kLanes;  // lanes along the channels (8 bytes each), groups of them along time
+
+template <typename io_t, int GRANULE, int S> struct Rows {
+  static constexpr int V = 8 / sizeof(io_t);
+  static constexpr int kGroupWords = S * kLanes;        // of 8 bytes
+  static constexpr int kWords = kGroups * kGroupWords;  // of a warp's rows
+
+  // A lane's 8 bytes of the rows of a group.
+  struct Mine {
+    const uint2 *even, *odd;
+    __device__ __forceinline__ Lanes<V> operator[](int i) const { return unpack<io_t>((i & 1 ? odd : even)[i * kLanes]); }
+  };
+  static __device__ __forceinline__ Mine mine(const uint2* space, int group) {
+    const uint2* at = space + group * kGroupWords + static_cast<int>(threadIdx.x) % kLanes;
+    const int swap = (group & 1) * kLanes;
+    return Mine{at + swap, at - swap};
+  }
+
+  // One access of GRANULE bytes; `bytes` of them exist.
+  static __device__ __forceinline__ void copy(unsigned to, const io_t* from, int bytes) {
+    if constexpr (GRANULE == 16)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" : : "r"(to), "l"(from), "r"(bytes) : "memory");
+    else
+      asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" : : "r"(to), "l"(from), "n"(GRANULE), "r"(bytes) : "memory");
+  }
+  // Rows [0, rows) of `base` + row * stride (for this warp), `channels` of the block's 8 * V.  FULL: all of them exist.
+  // `somewhere` is any valid address.
+  template <bool FULL>
+  static __device__ __forceinline__ void fetch(uint2* space, const io_t* base, long long stride, int rows, int channels, const io_t* somewhere) {
+    const int lane = threadIdx.x & 31;
     if constexpr (GRANULE == 2) {
-      alignas(8) io_t w[V];
+#pragma unroll 1
+      for (int i = 0; i < S; ++i) {
+        const int row = lane / kLanes * S + i, count = channels - lane % kLanes * V;
+        alignas(8) io_t w[V];
 #pragma unroll
-      for (int i = 0; i < V; ++i) w[i] = i < count ? from[i] : from_f32<io_t>(0.0f);
-      *to = *reinterpret_cast<const uint2*>(w);
+        for (int e = 0; e < V; ++e) w[e] = row < rows && e < count ? base[row * stride + lane % kLanes * V + e] : from_f32<io_t>(0.0f);
+        space[lane / kLanes * kGroupWords + (i ^ (lane / kLanes & 1)) * kLanes + lane % kLanes] = *reinterpret_cast<const uint2*>(w);
+      }
     } else {
-      const unsigned at = static_cast<unsigned>(__cvta_generic_to_shared(to));
+      constexpr int kParts = 64 / GRANULE, kRowsAtOnce = 32 / kParts;
+      static_assert(S % kRowsAtOnce == 0 && kRowsAtOnce % 2 == 0, "an access stays inside a group and holds whole pairs of rows");
+      const int part = lane % kParts, first = lane / kParts;  // kParts <= 16
+      const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(space)) + part * GRANULE;
+      const io_t* from = base + first * stride + part * (GRANULE / static_cast<int>(sizeof(io_t)));
+      const bool in = part * (GRANULE / static_cast<int>(sizeof(io_t))) < channels;
 #pragma unroll
-      for (int i = 0; i < 8 / GRANULE; ++i) {
-        const bool in = i * kElements < count;
-        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;"
-                     : : "r"(at + i * GRANULE), "l"(in ? from + i * kElements : from), "n"(GRANULE), "r"(in ? GRANULE : 0) : "memory");
+      for (int i = 0; i < kGroups * S / kRowsAtOnce; ++i) {
+        const int row = i * kRowsAtOnce + first;
+        const int group = i * kRowsAtOnce / S;  // the rows of one access are of one group
+        const unsigned at = to + group * kGroupWords * 8 + (i * kRowsAtOnce - group * S) * 64 + (first ^ (group & 1)) * 64;
+        if constexpr (FULL) {
+          copy(at, from, GRANULE);
+        } else {
+          const bool there = in && row < rows;
+          copy(at, there ? from : somewhere, there ? GRANULE : 0);
+        }
+        from += kRowsAtOnce * stride;
       }
     }
   }
-  static __device__ __forceinline__ void store(io_t* to, const Lanes<V>& a, int count) {
+  template <bool FULL> static __device__ __forceinline__ void store(io_t* to, const Lanes<V>& a, int count) {
     const uint2 w = pack<io_t>(a);
-    if constexpr (GRANULE == 8) {
-      if (count > 0) __stcs(reinterpret_cast<uint2*>(to), w);
+    if constexpr (GRANULE >= 8) {
+      if (FULL || count > 0) __stcs(reinterpret_cast<uint2*>(to), w);
     } else if constexpr (GRANULE == 4) {
-      if (count > 0) __stcs(reinterpret_cast<unsigned*>(to), w.x);
-      if (count > kElements) __stcs(reinterpret_cast<unsigned*>(to) + 1, w.y);
+      constexpr int kElements = 4 / sizeof(io_t);
+      if (FULL || count > 0) __stcs(reinterpret_cast<unsigned*>(to), w.x);
+      if (FULL || count > kElements) __stcs(reinterpret_cast<unsigned*>(to) + 1, w.y);
     } else {
       const io_t* e = reinterpret_cast<const io_t*>(&w);
 #pragma unroll
       for (int i = 0; i < V; ++i)
-        if (i < count) to[i] = e[i];
+        if (FULL || i < count) to[i] = e[i];
     }
   }
 };
