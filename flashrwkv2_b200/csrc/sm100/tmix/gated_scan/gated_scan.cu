@@ -19,15 +19,16 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kTile = 256;           // tokens of a CTA's tile
-constexpr int kForwardRows = 16, kBackwardRows = 8;  // tokens of a lane in a tile
-constexpr int kForwardWarps = kTile / (kGroups * kForwardRows), kBackwardWarps = kTile / (kGroups * kBackwardRows);
+constexpr int S = 16;                // tokens of a lane in a tile
+constexpr int kWarps = kTile / (kGroups * S), kThreads = kWarps * 32;
 // CTAs per SM.  Copies of 4 bytes go through L1, which the staging of a fourth CTA would leave too small for rows that lie
 // across its lines (16 x 1024 rows of 1003 fp32 channels: 86 us with four, 56 us with three).
 constexpr int forward_ctas(int granule) { return granule == 16 ? 4 : 3; }
 constexpr int kBackwardCtas = 2;
 constexpr int kMaxCluster = 8;
 constexpr int kShortRows = 16;       // sequences of at most this many tokens are served by the step kernel
-static_assert(kGroups * kBackwardRows == kSavedRows, "the backward pass loads a state for every warp");
+constexpr int kRanked = 128;         // up to this many sequences are taken longest first
+static_assert(S == kSavedRows, "the backward pass loads a state for every lane's rows");
 
 // NaN in every row that the call would write (fail-closed), by the whole grid.
 template <typename io_t>
@@ -66,11 +67,35 @@ struct Grid {
 
 __device__ __forceinline__ int row_begin(const GatedScanParams& p, int seq) { return p.cu != nullptr ? p.cu[seq] : seq * p.seq_len; }
 
-template <int V> __device__ __forceinline__ Unit unit_of(const GatedScanParams& p, const Grid& g, int unit, int n_seq) {
+// By all threads of the CTA.  Long sequences that start last would leave the GPU to a few CTAs, so a batch of a few
+// sequences of different lengths is taken longest first.  Each warp ranks them for itself and takes its answer from a vote:
+// the compiler then knows that the warp agrees, and what follows from it costs one lane, not 32 (64 x 2048 rows of 2560
+// channels: 317 us; with the answer read from shared memory 370).
+template <int V> __device__ __forceinline__ Unit unit_of(const GatedScanParams& p, const Grid& g, int unit, int n_seq, int* lengths) {
   const int lane = threadIdx.x & 31, chunk = unit / g.blocks;
   Unit u;
   u.first_seq = chunk * g.per_unit;
   u.channel = ((unit - chunk * g.blocks) * kLanes + lane % kLanes) * V;
+  if (p.cu != nullptr && g.per_unit == 1 && n_seq > 1 && n_seq <= kRanked) {
+    int longest = 0, shortest = 0x7fffffff;
+    for (int at = lane; at < n_seq; at += 32) {
+      const int len = p.cu[at + 1] - p.cu[at];
+      lengths[at] = len;  // every warp writes the same
+      longest = max(longest, len);
+      shortest = min(shortest, len);
+    }
+    if (__reduce_max_sync(0xffffffffu, longest) != __reduce_min_sync(0xffffffffu, shortest)) {
+      __syncwarp();
+      u.first_seq = n_seq;
+      for (int base = 0; base < n_seq; base += 32) {
+        const int at = base + lane, len = at < n_seq ? lengths[at] : -1;
+        int rank = 0;
+        for (int i = 0; i < n_seq; ++i) rank += lengths[i] > len || (lengths[i] == len && i < at);
+        const unsigned hit = __ballot_sync(0xffffffffu, at < n_seq && rank == chunk);
+        if (hit != 0) u.first_seq = base + __ffs(hit) - 1;
+      }
+    }
+  }
   const int seq = u.first_seq + lane;
   const bool mine = lane < g.per_unit && seq < n_seq && row_begin(p, seq + 1) - row_begin(p, seq) > p.longer_than;
   u.left = __ballot_sync(0xffffffffu, mine);
@@ -104,20 +129,31 @@ template <int V> struct Scan {
   }
 };
 
+// The maps of one warp's or CTA's rows in shared memory, by lane along the channels.
+template <int V> struct Pieces {
+  Lanes<V> a[kLanes], b[kLanes];
+
+  __device__ __forceinline__ void put(const Map<V>& m) {
+    a[threadIdx.x % kLanes] = m.a;
+    b[threadIdx.x % kLanes] = m.b;
+  }
+  __device__ __forceinline__ Map<V> get() const { return Map<V>{a[threadIdx.x % kLanes], b[threadIdx.x % kLanes]}; }
+};
+
 // Joins the CTAs of a cluster: each writes its map into everyone's shared memory (slots[rank]), a cluster barrier, and each
 // applies the maps of the ranks before it.  Returns the state before this CTA's tile and moves `carry` behind the cluster's.
 template <int V>
-__device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Map<V> (*slots)[kLanes], Lanes<V>& carry) {
+__device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Pieces<V>* slots, Lanes<V>& carry) {
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   for (int r = warp; r < ranks; r += static_cast<int>(blockDim.x) / 32)
-    if (lane < kLanes) cluster.map_shared_rank(&slots[rank][0], r)[lane] = cta;
+    if (lane < kLanes) cluster.map_shared_rank(&slots[rank], r)->put(cta);
   cluster.sync();
   Lanes<V> mine = carry;
   for (int r = 0; r < ranks; ++r) {
     if (r == rank) mine = carry;
-    carry = slots[r][lane % kLanes].apply(carry);
+    carry = slots[r].get().apply(carry);
   }
   return mine;
 }
@@ -125,13 +161,14 @@ __device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Map<V> (*slo
 // ---- forward
 
 template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kForwardWarps * 32, forward_ctas(GRANULE)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
-  constexpr int V = 8 / sizeof(io_t), S = kForwardRows, kWarps = kForwardWarps;
+__global__ void __launch_bounds__(kThreads, forward_ctas(GRANULE)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
+  constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
   using R = Rows<io_t, GRANULE, S>;
   extern __shared__ uint2 staged[];  // x of two tiles, then the decays of one: [warp][R::kWords]
-  __shared__ Map<V> pieces[2][kWarps][kLanes], slots[2][CLUSTER ? kMaxCluster : 1][kLanes];
+  __shared__ int lengths[kRanked];
+  __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, p.boundary != nullptr ? p.final_state : nullptr, p.n_seq);
@@ -140,7 +177,7 @@ __global__ void __launch_bounds__(kForwardWarps * 32, forward_ctas(GRANULE)) gat
   if constexpr (CLUSTER) cg::this_cluster().sync();  // everyone's shared memory is there before it is written to
   const int n_seq = p.status != nullptr ? p.status[2] : p.n_seq;
   const int ranks = CLUSTER ? grid.cluster : 1, rank = CLUSTER ? static_cast<int>(blockIdx.x) % ranks : 0;
-  Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, n_seq);
+  Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, n_seq, lengths);
   const int channel = unit.channel, count = min(V, p.channels - channel);
   const int block_channel = channel - lane % kLanes * V, block_count = min(kLanes * V, p.channels - block_channel);
   const auto first_tile = [&](int seq) {
@@ -207,28 +244,31 @@ __global__ void __launch_bounds__(kForwardWarps * 32, forward_ctas(GRANULE)) gat
     __syncwarp();  // the decays have been read: their place is free
     fetch(next, buffer ^ 1);  // in flight while this tile is joined and written
     const Map<V> before = Scan<V>::join_groups(map);
-    if (lane >= 32 - kLanes) pieces[buffer][warp][lane % kLanes] = map;
+    if (lane >= 32 - kLanes) pieces[buffer][warp].put(map);
     __syncthreads();
 
     // the state before this warp's rows, and behind the tile
     L h = carry;
     if constexpr (CLUSTER) {
-      Map<V> cta = pieces[buffer][0][lane % kLanes];
+      Map<V> cta = pieces[buffer][0].get();
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w][lane % kLanes]);
+      for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w].get());
       h = join_cluster<V>(cta, slots[buffer], carry);
-      for (int w = 0; w < warp; ++w) h = pieces[buffer][w][lane % kLanes].apply(h);
+      for (int w = 0; w < warp; ++w) h = pieces[buffer][w].get().apply(h);
     } else {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w == warp) h = carry;
-        carry = pieces[buffer][w][lane % kLanes].apply(carry);
+        carry = pieces[buffer][w].get().apply(carry);
       }
     }
     h = before.apply(h);
     const int left = tile.len - tile.at - own;
-    if (p.boundary != nullptr && own % kSavedRows == 0 && left > 0)
-      store_states<V>(p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel, h, count);
+    if (p.boundary != nullptr && left > 0) {
+      float* to = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;
+      if (GRANULE == 16 && count == V) store_states_whole<V>(to, h);
+      else store_states<V>(to, h, count);
+    }
     if (next.seq != tile.seq) carry = initial_state(next);
 
     // second sweep
@@ -326,17 +366,18 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
 // With c_t = rho_t g_t the same recurrence runs against time: g_t = dy_t + c_{t+1}, and c behind the last token is the final
 // state's gradient.  Steps go from the end of a sequence to its start and rank 0 of a cluster takes the last of a step's
 // tiles; inside a tile warps, lane groups and rows are counted from its end, so that all joins are those of the forward
-// pass.  The states come from those that the forward pass saved before every warp's rows.
+// pass.  The states come from those that the forward pass saved before every lane's rows.
 
 template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kBackwardWarps * 32, kBackwardCtas)
+__global__ void __launch_bounds__(kThreads, kBackwardCtas)
 gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const Grid grid) {
-  constexpr int V = 8 / sizeof(io_t), S = kBackwardRows, kWarps = kBackwardWarps, kWarpRows = kGroups * S;
+  constexpr int V = 8 / sizeof(io_t), kWarpRows = kGroups * S;
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
   using R = Rows<io_t, GRANULE, S>;
   extern __shared__ uint2 staged[];  // [2 tiles][x, decay or dy][warp][R::kWords]
-  __shared__ Map<V> pieces[2][kWarps][kLanes], slots[2][CLUSTER ? kMaxCluster : 1][kLanes];
+  __shared__ int lengths[kRanked];
+  __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(g.dx), static_cast<io_t*>(g.ddecay), g.dinitial, p.n_seq);
@@ -344,7 +385,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   }
   if constexpr (CLUSTER) cg::this_cluster().sync();
   const int ranks = CLUSTER ? grid.cluster : 1, rank = CLUSTER ? static_cast<int>(blockIdx.x) % ranks : 0;
-  Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, p.n_seq);
+  Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, p.n_seq, lengths);
   const int channel = unit.channel, count = min(V, p.channels - channel);
   const int block_channel = channel - lane % kLanes * V, block_count = min(kLanes * V, p.channels - block_channel);
   const int step_rows = ranks * kTile;
@@ -388,69 +429,60 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   for (int round = 0; tile.seq >= 0; ++round) {
     const int buffer = round & 1, left = tile.len - tile.at - own;
     const Tile next = tile_after(tile);
-    // the state before this warp's rows, where it has any
-    const int warp_at = tile.at + warp_row;
-    const L saved = warp_at < tile.len
-                        ? load_states<V>(p.boundary + saved_row(tile.seq, tile.begin, warp_at) * p.channels + channel, count)
-                        : L::all(0.0f);
+    // the state before this lane's rows, where it has any
+    L h = L::all(0.0f);
+    if (left > 0) {
+      const float* from = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;
+      h = GRANULE == 16 && count == V ? load_states_whole<V>(from) : load_states<V>(from, count);
+    }
     copies_done();
     __syncwarp();  // what the warp's other lanes copied
     const typename R::Mine x = R::mine(space(buffer, 0), group), d = R::mine(space(buffer, 1), group),
                            dy = R::mine(space(buffer, 2), group);
 
-    // first sweep: the gates, and the maps of h (rows in time) and c (against it).  Rows behind the sequence's end leave c as
-    // it is.
-    L kept[S];
-    Map<V> map = Map<V>::identity(), back = map;
-#pragma unroll
-    for (int i = 0; i < S; ++i) {
-      kept[i] = D::keep(d[i], L::all(0.0f));
-      map.b = D::step(kept[i], map.b, x[i]);
-      if (i < left) map.a = D::fade(kept[i], map.a);
-    }
-#pragma unroll
-    for (int i = S - 1; i >= 0; --i) {
-      if (i < left) back.b = D::fade(kept[i], add(dy[i], back.b));
-    }
-    back.a = map.a;
-    const Map<V> behind = Scan<V>::join_groups(back);
-    if (lane >= 32 - kLanes) pieces[buffer][warp][lane % kLanes] = back;
-    // h before this lane's rows: lane groups are counted against time, so their maps come from the lanes above
-    L h = saved;
-#pragma unroll
-    for (int gr = kGroups - 1; gr > 0; --gr) {
-      Map<V> m;
-#pragma unroll
-      for (int i = 0; i < V / 2; ++i) {
-        const int from = gr * kLanes + lane % kLanes;
-        m.a.v[i] = make_float2(__shfl_sync(0xffffffffu, map.a.v[i].x, from), __shfl_sync(0xffffffffu, map.a.v[i].y, from));
-        m.b.v[i] = make_float2(__shfl_sync(0xffffffffu, map.b.v[i].x, from), __shfl_sync(0xffffffffu, map.b.v[i].y, from));
-      }
-      if (lane / kLanes < gr) h = m.apply(h);
-    }
-    // what ddecay needs of the states: the state before every row, less its input (complement)
-    L states[S];
+    // with time: the gates, and what a row's gradient is multiplied by for ddecay: the state before it, less its input
+    // (complement), by the gate's slope
+    L kept[S], states[S];
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const L value = x[i];
+      L sigmoid;
+      if constexpr (LOGITS) {
+        sigmoid = D::sigmoid(d[i], L::all(0.0f));
+        kept[i] = D::keep_gate(sigmoid);
+      } else {
+        kept[i] = d[i];
+      }
       states[i] = COMPLEMENT ? minus(h, value) : h;
+      if constexpr (LOGITS) states[i] = mul(states[i], D::slope(sigmoid, kept[i]));
       h = D::step(kept[i], h, value);
     }
+    // against it: the map of c.  Rows behind the sequence's end leave c as it is.
+    Map<V> back = Map<V>::identity();
+#pragma unroll
+    for (int i = S - 1; i >= 0; --i) {
+      if (i < left) {
+        back.b = D::fade(kept[i], add(dy[i], back.b));
+        back.a = D::fade(kept[i], back.a);
+      }
+    }
+    const Map<V> behind = Scan<V>::join_groups(back);
+    if (lane >= 32 - kLanes) pieces[buffer][warp].put(back);
     fetch(next, buffer ^ 1);
     __syncthreads();
 
     L c = carry;
     if constexpr (CLUSTER) {
-      Map<V> cta = pieces[buffer][0][lane % kLanes];
+      Map<V> cta = pieces[buffer][0].get();
 #pragma unroll
-      for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w][lane % kLanes]);
+      for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w].get());
       c = join_cluster<V>(cta, slots[buffer], carry);
-      for (int w = 0; w < warp; ++w) c = pieces[buffer][w][lane % kLanes].apply(c);
+      for (int w = 0; w < warp; ++w) c = pieces[buffer][w].get().apply(c);
     } else {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         if (w == warp) c = carry;
-        carry = pieces[buffer][w][lane % kLanes].apply(carry);
+        carry = pieces[buffer][w].get().apply(carry);
       }
     }
     c = behind.apply(c);
@@ -467,9 +499,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
           const L grad = add(dy[i], c);
           c = D::fade(kept[i], grad);
           R::template store<full()>(dx, D::input_grad(kept[i], grad), count);
-          L drho = mul(grad, states[i]);
-          if constexpr (LOGITS) drho = mul(drho, D::slope(D::sigmoid(d[i], L::all(0.0f)), kept[i]));
-          R::template store<full()>(dd, drho, count);
+          R::template store<full()>(dd, mul(grad, states[i]), count);
         }
         dx -= p.channels;
         dd -= p.channels;
@@ -574,10 +604,10 @@ Grid cut(const GatedScanParams& p, int max_seqlen, int lanes, int slots) {
 }
 
 template <typename K, typename... Args>
-int launch(K kernel, const Grid& g, const GatedScanParams& p, int warps, int words, void* stream, const char* what, Args... args) {
+int launch(K kernel, const Grid& g, const GatedScanParams& p, int words, void* stream, const char* what, Args... args) {
   const long long units = static_cast<long long>((p.n_seq + g.per_unit - 1) / g.per_unit) * g.blocks;
   if (units * g.cluster > 0x7fffffffll) return fail(FRWKV_ERR_UNSUPPORTED, "%s: too many sequences by channels", what);
-  const int shared = warps * words * 8;
+  const int shared = kWarps * words * 8;
   const cudaError_t error = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
   if (error != cudaSuccess) return fail(FRWKV_ERR_CUDA, "%s: preparing the launch: %s", what, cudaGetErrorString(error));
   cudaLaunchAttribute cluster;
@@ -586,7 +616,7 @@ int launch(K kernel, const Grid& g, const GatedScanParams& p, int warps, int wor
   cluster.val.clusterDim.y = cluster.val.clusterDim.z = 1;
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(units * g.cluster));
-  config.blockDim = dim3(static_cast<unsigned>(warps) * 32);
+  config.blockDim = dim3(kThreads);
   config.dynamicSmemBytes = static_cast<size_t>(shared);
   config.stream = static_cast<cudaStream_t>(stream);
   config.attrs = &cluster;
@@ -597,14 +627,14 @@ int launch(K kernel, const Grid& g, const GatedScanParams& p, int warps, int wor
 
 int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream) {
   int rc = FRWKV_OK;
-  with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y}), [&](auto io, auto granule) {
+  with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y, p.boundary}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
       const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(granule()) * sm_count());
-      constexpr int kWords = 3 * Rows<io_t, granule(), kForwardRows>::kWords;
+      constexpr int kWords = 3 * Rows<io_t, granule(), S>::kWords;
       constexpr const char* kName = "gated_scan_forward_kernel";
-      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), true>, g, p, kForwardWarps, kWords, stream, kName)
-                         : launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), false>, g, p, kForwardWarps, kWords, stream, kName);
+      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), true>, g, p, kWords, stream, kName)
+                         : launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), false>, g, p, kWords, stream, kName);
     });
   });
   return rc;
@@ -689,14 +719,14 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
                           total_tokens / n_seq, 0};
   const GatedScanGrads g{dy, dfinal, dx, ddecay, dinitial};
   int rc = FRWKV_OK;
-  with_type(io_dtype, granule_of(p, io_dtype, {x, decay, dy, dx, ddecay}), [&](auto io, auto granule) {
+  with_type(io_dtype, granule_of(p, io_dtype, {x, decay, dy, dx, ddecay, boundary}), [&](auto io, auto granule) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
       const Grid grid = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kBackwardCtas * sm_count());
-      constexpr int kWords = 6 * Rows<io_t, granule(), kBackwardRows>::kWords;
+      constexpr int kWords = 6 * Rows<io_t, granule(), S>::kWords;
       constexpr const char* kName = "gated_scan_backward_kernel";
-      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), true>, grid, p, kBackwardWarps, kWords, stream, kName, g)
-                            : launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), false>, grid, p, kBackwardWarps, kWords, stream, kName, g);
+      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), true>, grid, p, kWords, stream, kName, g)
+                            : launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), false>, grid, p, kWords, stream, kName, g);
     });
   });
   return rc;

@@ -41,7 +41,7 @@ struct GatedScanGrads {
 
 // ---- the channels of a lane: 8 bytes of a token row, in pairs for packed fp32 arithmetic
 
-template <int V> struct Lanes {
+template <int V> struct alignas(4 * V) Lanes {
   float2 v[V / 2];
 
   static __device__ __forceinline__ Lanes all(float x) {
@@ -206,6 +206,23 @@ template <int V> __device__ __forceinline__ void store_states(float* to, const L
   }
 }
 
+// The same where a lane's states are known to exist and to be aligned to their size.
+template <int V> __device__ __forceinline__ Lanes<V> load_states_whole(const float* from) {
+  Lanes<V> r;
+  if constexpr (V == 4) {
+    const float4 w = __ldcs(reinterpret_cast<const float4*>(from));
+    r.v[0] = make_float2(w.x, w.y);
+    r.v[1] = make_float2(w.z, w.w);
+  } else {
+    r.v[0] = __ldcs(reinterpret_cast<const float2*>(from));
+  }
+  return r;
+}
+template <int V> __device__ __forceinline__ void store_states_whole(float* to, const Lanes<V>& a) {
+  if constexpr (V == 4) __stcs(reinterpret_cast<float4*>(to), make_float4(a.v[0].x, a.v[0].y, a.v[1].x, a.v[1].y));
+  else __stcs(reinterpret_cast<float2*>(to), a.v[0]);
+}
+
 // ---- gate
 
 // What a token does to the state.  LOGITS keeps rho - 1, otherwise rho is kept (see the top of the file).
@@ -261,7 +278,7 @@ template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
 
 // ---- affine maps h -> a h + b
 
-template <int V> struct alignas(4 * V) Map {
+template <int V> struct Map {
   Lanes<V> a, b;
 
   static __device__ __forceinline__ Map identity() { return Map{Lanes<V>::all(1.0f), Lanes<V>::all(0.0f)}; }

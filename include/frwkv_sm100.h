@@ -262,7 +262,7 @@ int frwkv_sm100_gated_scan(
  *              state before every FRWKV_GATED_SCAN_SAVED_ROWS-th token of every sequence;
  *   max_seqlen : largest sequence length of packed rows (a launch-shape hint; <= 0 if unknown);
  *   dy, dx, ddecay : contiguous, token dtype;  dfinal (NULL: zeros), dinitial (NULL: not wanted) : fp32. */
-#define FRWKV_GATED_SCAN_SAVED_ROWS 32
+#define FRWKV_GATED_SCAN_SAVED_ROWS 16
 int frwkv_sm100_gated_scan_train_forward(
     const int32_t* cu_seqlens, const int32_t* status, const void* x, long long x_row_stride, const void* decay,
     long long decay_row_stride, const float* initial, void* y, float* final_state, float* boundary, int n_seq,
