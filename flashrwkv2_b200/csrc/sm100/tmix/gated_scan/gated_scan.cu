@@ -21,9 +21,8 @@ namespace cg = cooperative_groups;
 constexpr int kTile = 256;           // tokens of a CTA's tile
 constexpr int S = 16;                // tokens of a lane in a tile
 constexpr int kWarps = kTile / (kGroups * S), kThreads = kWarps * 32;
-// CTAs per SM.  Copies of 4 bytes go through L1, which the staging of a fourth CTA would leave too small for rows that lie
-// across its lines (16 x 1024 rows of 1003 fp32 channels: 86 us with four, 56 us with three).
-constexpr int forward_ctas(int granule) { return granule == 16 ? 4 : 3; }
+// CTAs per SM, by registers and by the staging of their rows
+constexpr int forward_ctas(bool aligned) { return aligned ? 4 : 3; }
 constexpr int kBackwardCtas = 2;
 constexpr int kMaxCluster = 8;
 constexpr int kShortRows = 16;       // sequences of at most this many tokens are served by the step kernel
@@ -160,12 +159,12 @@ __device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Pieces<V>* s
 
 // ---- forward
 
-template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, forward_ctas(GRANULE)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
+template <typename io_t, bool ALIGNED, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
-  using R = Rows<io_t, GRANULE, S>;
+  using R = Rows<io_t, ALIGNED, S>;
   extern __shared__ uint2 staged[];  // x of two tiles, then the decays of one: [warp][R::kWords]
   __shared__ int lengths[kRanked];
   __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
@@ -189,7 +188,9 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(GRANULE)) gated_scan_fo
     const int at = t.at + ranks * kTile;
     return at - rank * kTile < t.len ? Tile{t.seq, t.begin, at, t.len} : first_tile(unit.next());
   };
-  const auto is_full = [&](const Tile& t) { return t.at + kTile <= t.len && block_count == kLanes * V; };
+  const auto is_full = [&](const Tile& t) {
+    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || t.begin + t.at > 0);
+  };
   const int warp_row = warp * kGroups * S, own = warp_row + lane / kLanes * S;  // first rows in a tile
   uint2* const decays = staged + (2 * kWarps + warp) * R::kWords;
   const auto inputs = [&](int buffer) { return staged + (buffer * kWarps + warp) * R::kWords; };
@@ -232,7 +233,9 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(GRANULE)) gated_scan_fo
     __syncwarp();  // what the warp's other lanes copied
 
     // first sweep: the gates into registers, and the map of this lane's rows
-    const typename R::Mine x = R::mine(inputs(buffer), lane / kLanes), d = R::mine(decays, lane / kLanes);
+    const long long own_row = tile.begin + tile.at + own;
+    const typename R::Mine x = R::mine(inputs(buffer), lane / kLanes, static_cast<const io_t*>(p.x) + own_row * p.x_stride + block_channel, p.x_stride);
+    const typename R::Mine d = R::mine(decays, lane / kLanes, static_cast<const io_t*>(p.decay) + own_row * p.decay_stride + block_channel, p.decay_stride);
     L kept[S];
     Map<V> map = Map<V>::identity();
 #pragma unroll
@@ -266,13 +269,13 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(GRANULE)) gated_scan_fo
     const int left = tile.len - tile.at - own;
     if (p.boundary != nullptr && left > 0) {
       float* to = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;
-      if (GRANULE == 16 && count == V) store_states_whole<V>(to, h);
+      if (ALIGNED && count == V) store_states_whole<V>(to, h);
       else store_states<V>(to, h, count);
     }
     if (next.seq != tile.seq) carry = initial_state(next);
 
     // second sweep
-    io_t* y = static_cast<io_t*>(p.y) + static_cast<long long>(tile.begin + tile.at + own) * p.channels + channel;
+    io_t* y = static_cast<io_t*>(p.y) + own_row * p.channels + channel;
     if (is_full(tile)) {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
@@ -368,14 +371,14 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
 // tiles; inside a tile warps, lane groups and rows are counted from its end, so that all joins are those of the forward
 // pass.  The states come from those that the forward pass saved before every lane's rows.
 
-template <typename io_t, int GRANULE, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
+template <typename io_t, bool ALIGNED, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas)
 gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t), kWarpRows = kGroups * S;
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
-  using R = Rows<io_t, GRANULE, S>;
-  extern __shared__ uint2 staged[];  // [2 tiles][x, decay or dy][warp][R::kWords]
+  using R = Rows<io_t, ALIGNED, S>;
+  extern __shared__ uint2 staged[];  // x and the decays of one tile, then dy of two: [warp][R::kWords]
   __shared__ int lengths[kRanked];
   __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -397,11 +400,13 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   const auto tile_after = [&](const Tile& t) {
     return t.at >= step_rows ? Tile{t.seq, t.begin, t.at - step_rows, t.len} : first_tile(unit.next());
   };
-  const auto is_full = [&](const Tile& t) { return t.at + kTile <= t.len && block_count == kLanes * V; };
+  const auto is_full = [&](const Tile& t) {
+    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || t.begin + t.at > 0);
+  };
   // In memory the lane groups of a warp lie as in the forward pass, first in time first; along the chain a lane works on
   // group kGroups - 1 - lane / kLanes.
   const int warp_row = (kWarps - 1 - warp) * kWarpRows, group = kGroups - 1 - lane / kLanes, own = warp_row + group * S;
-  const auto space = [&](int buffer, int tensor) { return staged + ((buffer * 3 + tensor) * kWarps + warp) * R::kWords; };
+  const auto space = [&](int i) { return staged + (i * kWarps + warp) * R::kWords; };
   const auto fetch = [&](const Tile& t, int buffer) {
     if (t.seq < 0) return;
     const int row = t.begin + t.at + warp_row, left = t.len - t.at - warp_row;
@@ -409,13 +414,13 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     const io_t *x_rows = x + row * p.x_stride + block_channel, *d_rows = d + row * p.decay_stride + block_channel;
     const io_t* dy_rows = dy + static_cast<long long>(row) * p.channels + block_channel;
     if (is_full(t)) {
-      R::template fetch<true>(space(buffer, 0), x_rows, p.x_stride, left, block_count, x);
-      R::template fetch<true>(space(buffer, 1), d_rows, p.decay_stride, left, block_count, d);
-      R::template fetch<true>(space(buffer, 2), dy_rows, p.channels, left, block_count, dy);
+      R::template fetch<true>(space(0), x_rows, p.x_stride, left, block_count, x);
+      R::template fetch<true>(space(1), d_rows, p.decay_stride, left, block_count, d);
+      R::template fetch<true>(space(2 + buffer), dy_rows, p.channels, left, block_count, dy);
     } else {
-      R::template fetch<false>(space(buffer, 0), x_rows, p.x_stride, left, block_count, x);
-      R::template fetch<false>(space(buffer, 1), d_rows, p.decay_stride, left, block_count, d);
-      R::template fetch<false>(space(buffer, 2), dy_rows, p.channels, left, block_count, dy);
+      R::template fetch<false>(space(0), x_rows, p.x_stride, left, block_count, x);
+      R::template fetch<false>(space(1), d_rows, p.decay_stride, left, block_count, d);
+      R::template fetch<false>(space(2 + buffer), dy_rows, p.channels, left, block_count, dy);
     }
     copies_begun();
   };
@@ -433,12 +438,14 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     L h = L::all(0.0f);
     if (left > 0) {
       const float* from = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;
-      h = GRANULE == 16 && count == V ? load_states_whole<V>(from) : load_states<V>(from, count);
+      h = ALIGNED && count == V ? load_states_whole<V>(from) : load_states<V>(from, count);
     }
     copies_done();
     __syncwarp();  // what the warp's other lanes copied
-    const typename R::Mine x = R::mine(space(buffer, 0), group), d = R::mine(space(buffer, 1), group),
-                           dy = R::mine(space(buffer, 2), group);
+    const long long own_row = tile.begin + tile.at + own;
+    const typename R::Mine x = R::mine(space(0), group, static_cast<const io_t*>(p.x) + own_row * p.x_stride + block_channel, p.x_stride);
+    const typename R::Mine d = R::mine(space(1), group, static_cast<const io_t*>(p.decay) + own_row * p.decay_stride + block_channel, p.decay_stride);
+    const typename R::Mine dy = R::mine(space(2 + buffer), group, static_cast<const io_t*>(g.dy) + own_row * p.channels + block_channel, p.channels);
 
     // with time: the gates, and what a row's gradient is multiplied by for ddecay: the state before it, less its input
     // (complement), by the gate's slope
@@ -468,6 +475,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     }
     const Map<V> behind = Scan<V>::join_groups(back);
     if (lane >= 32 - kLanes) pieces[buffer][warp].put(back);
+    __syncwarp();  // the inputs and the decays have been read: their place is free
     fetch(next, buffer ^ 1);
     __syncthreads();
 
@@ -489,9 +497,8 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     if (next.seq != tile.seq) carry = final_grad(next);
 
     // second sweep
-    const long long row = tile.begin + tile.at + own;
-    io_t* dx = static_cast<io_t*>(g.dx) + (row + S - 1) * p.channels + channel;
-    io_t* dd = static_cast<io_t*>(g.ddecay) + (row + S - 1) * p.channels + channel;
+    io_t* dx = static_cast<io_t*>(g.dx) + (own_row + S - 1) * p.channels + channel;
+    io_t* dd = static_cast<io_t*>(g.ddecay) + (own_row + S - 1) * p.channels + channel;
     const auto sweep = [&](auto full) {
 #pragma unroll
       for (int i = S - 1; i >= 0; --i) {
@@ -507,7 +514,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     };
     if (is_full(tile)) sweep(std::true_type{});
     else sweep(std::false_type{});
-    __syncwarp();  // everything has been read: the place is free
+    __syncwarp();  // dy has been read
     if (tile.at + own == 0 && g.dinitial != nullptr)
       store_states<V>(g.dinitial + static_cast<long long>(tile.seq) * p.channels + channel, c, count);
     tile = next;
@@ -559,25 +566,18 @@ template <typename F> void with_modes(int decay_mode, int input_mode, F f) {
   }
 }
 
-// Calls f with the token type and the largest access that fits everything as compile-time constants.
-template <typename F> void with_type(int io_dtype, int granule, F f) {
-  using two = std::integral_constant<int, 2>;
-  using four = std::integral_constant<int, 4>;
-  using all = std::integral_constant<int, 16>;
-  if (io_dtype == FRWKV_IO_FP32) granule == 16 ? f(float{}, all{}) : f(float{}, four{});
-  else if (io_dtype == FRWKV_IO_BF16) granule == 16 ? f(__nv_bfloat16{}, all{}) : granule == 4 ? f(__nv_bfloat16{}, four{}) : f(__nv_bfloat16{}, two{});
-  else granule == 16 ? f(__half{}, all{}) : granule == 4 ? f(__half{}, four{}) : f(__half{}, two{});
+// Calls f with the token type, and whether all rows begin at multiples of 16 bytes, as compile-time constants.
+template <typename F> void with_type(int io_dtype, bool aligned, F f) {
+  using yes = std::true_type;
+  using no = std::false_type;
+  if (io_dtype == FRWKV_IO_FP32) aligned ? f(float{}, yes{}) : f(float{}, no{});
+  else if (io_dtype == FRWKV_IO_BF16) aligned ? f(__nv_bfloat16{}, yes{}) : f(__nv_bfloat16{}, no{});
+  else aligned ? f(__half{}, yes{}) : f(__half{}, no{});
 }
 
-// The bytes of a token row that one access may move: 16 where the channels, the strides and all starts allow it, else 4, or
-// a 16-bit element.
-int granule_of(const GatedScanParams& p, int io_dtype, std::initializer_list<const void*> rows) {
-  const int element = io_dtype == FRWKV_IO_FP32 ? 4 : 2;
-  for (int granule : {16, 4}) {
-    const int n = granule / element;
-    if (p.channels % n == 0 && p.x_stride % n == 0 && p.decay_stride % n == 0 && multiple_of(granule, rows)) return granule;
-  }
-  return 2;
+bool rows_aligned(const GatedScanParams& p, int io_dtype, std::initializer_list<const void*> rows) {
+  const int n = io_dtype == FRWKV_IO_FP32 ? 4 : 8;
+  return p.channels % n == 0 && p.x_stride % n == 0 && p.decay_stride % n == 0 && multiple_of(16, rows);
 }
 
 // How the work is cut.  Few sequences with few channels leave the GPU empty, so a cluster shares a sequence: the size that
@@ -627,14 +627,14 @@ int launch(K kernel, const Grid& g, const GatedScanParams& p, int words, void* s
 
 int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream) {
   int rc = FRWKV_OK;
-  with_type(io_dtype, granule_of(p, io_dtype, {p.x, p.decay, p.y, p.boundary}), [&](auto io, auto granule) {
+  with_type(io_dtype, rows_aligned(p, io_dtype, {p.x, p.decay, p.y, p.boundary}), [&](auto io, auto aligned) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
-      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(granule()) * sm_count());
-      constexpr int kWords = 3 * Rows<io_t, granule(), S>::kWords;
+      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(aligned()) * sm_count());
+      constexpr int kWords = 3 * Rows<io_t, aligned(), S>::kWords;
       constexpr const char* kName = "gated_scan_forward_kernel";
-      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), true>, g, p, kWords, stream, kName)
-                         : launch(gated_scan_forward_kernel<io_t, granule(), logits(), complement(), false>, g, p, kWords, stream, kName);
+      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, aligned(), logits(), complement(), true>, g, p, kWords, stream, kName)
+                         : launch(gated_scan_forward_kernel<io_t, aligned(), logits(), complement(), false>, g, p, kWords, stream, kName);
     });
   });
   return rc;
@@ -719,14 +719,14 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
                           total_tokens / n_seq, 0};
   const GatedScanGrads g{dy, dfinal, dx, ddecay, dinitial};
   int rc = FRWKV_OK;
-  with_type(io_dtype, granule_of(p, io_dtype, {x, decay, dy, dx, ddecay, boundary}), [&](auto io, auto granule) {
+  with_type(io_dtype, rows_aligned(p, io_dtype, {x, decay, dy, dx, ddecay, boundary}), [&](auto io, auto aligned) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
       const Grid grid = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kBackwardCtas * sm_count());
-      constexpr int kWords = 6 * Rows<io_t, granule(), S>::kWords;
+      constexpr int kWords = 4 * Rows<io_t, aligned(), S>::kWords;
       constexpr const char* kName = "gated_scan_backward_kernel";
-      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), true>, grid, p, kWords, stream, kName, g)
-                            : launch(gated_scan_backward_kernel<io_t, granule(), logits(), complement(), false>, grid, p, kWords, stream, kName, g);
+      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, aligned(), logits(), complement(), true>, grid, p, kWords, stream, kName, g)
+                            : launch(gated_scan_backward_kernel<io_t, aligned(), logits(), complement(), false>, grid, p, kWords, stream, kName, g);
     });
   });
   return rc;
