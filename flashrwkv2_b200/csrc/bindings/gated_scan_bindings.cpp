@@ -121,9 +121,14 @@ std::tuple<int64_t, Optional, Optional> resolve_rows(const RowsShape& s, const t
   return {n, prepared.cu, prepared.status};
 }
 
-py::tuple pretrain_tmix_gated_scan_forward(const torch::Tensor& x, const torch::Tensor& decay_logits,
-                                           const Optional& initial_state, const Optional& cu_seqlens,
-                                           const std::string& decay_mode, const std::string& input_mode) {
+struct Forward {
+  torch::Tensor y, final_state, boundary;
+  Optional cu, status;
+};
+
+Forward train_forward(const torch::Tensor& x, const torch::Tensor& decay_logits,
+                      const Optional& initial_state, const Optional& cu_seqlens, const std::string& decay_mode,
+                      const std::string& input_mode) {
   const int mode = decay_code_checked(decay_mode), input = input_code(input_mode);
   if (cu_seqlens.has_value()) {
     need_type(cu_seqlens->scalar_type() == torch::kInt32, "cu_seqlens must have dtype int32");
@@ -150,11 +155,10 @@ py::tuple pretrain_tmix_gated_scan_forward(const torch::Tensor& x, const torch::
       static_cast<const float*>(optional_pointer(initial_state)), y.data_ptr(), final_state.data_ptr<float>(),
       boundary.data_ptr<float>(), static_cast<int>(n), static_cast<int>(s.total), static_cast<int>(s.channels),
       io_code(x), mode, input, -1, at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
-  return py::make_tuple(y, final_state, boundary, cu, status);
+  return Forward{y, final_state, boundary, cu, status};
 }
 
-py::tuple pretrain_tmix_gated_scan_backward(const torch::Tensor& x, const torch::Tensor& decay_logits,
-                                            const Optional& initial_state, const Optional& cu, const Optional& status,
+torch::autograd::variable_list train_backward(const torch::Tensor& x, const torch::Tensor& decay_logits, const Optional& initial_state, const Optional& cu, const Optional& status,
                                             const torch::Tensor& boundary, const torch::Tensor& grad_output,
                                             const Optional& grad_final, const std::string& decay_mode,
                                             const std::string& input_mode) {
@@ -181,7 +185,49 @@ py::tuple pretrain_tmix_gated_scan_backward(const torch::Tensor& x, const torch:
       static_cast<float*>(optional_pointer(dinitial)), static_cast<int>(n), static_cast<int>(s.total),
       static_cast<int>(s.channels), io_code(x), mode, input, -1,
       at::cuda::getCurrentCUDAStream(x.device().index()).stream()));
-  return py::make_tuple(dx, ddecay, dinitial);
+  return {dx, ddecay, dinitial.value_or(torch::Tensor())};
+}
+
+Optional defined(const torch::Tensor& t) { return t.defined() ? Optional(t) : std::nullopt; }
+
+class TrainFunction : public torch::autograd::Function<TrainFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& x,
+                                                const torch::Tensor& decay_logits, const Optional& initial_state,
+                                                const Optional& cu_seqlens, const std::string& decay_mode,
+                                                const std::string& input_mode) {
+    const Forward f = train_forward(x, decay_logits, initial_state, cu_seqlens, decay_mode, input_mode);
+    ctx->save_for_backward({x, decay_logits, initial_state.value_or(torch::Tensor()), f.cu.value_or(torch::Tensor()), f.status.value_or(torch::Tensor()), f.boundary});
+    ctx->saved_data["decay_mode"] = decay_mode;
+    ctx->saved_data["input_mode"] = input_mode;
+    ctx->set_materialize_grads(false);
+    return {f.y, f.final_state};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto& x = saved[0];
+    const auto grad_output = grads[0].defined() ? grads[0].contiguous() : torch::zeros(x.sizes(), x.options());
+    const auto grad_final = grads[1].defined() ? Optional(grads[1].contiguous()) : std::nullopt;
+    auto out = train_backward(x, saved[1], defined(saved[2]), defined(saved[3]), defined(saved[4]), saved[5], grad_output, grad_final,
+                              ctx->saved_data["decay_mode"].toStringRef(), ctx->saved_data["input_mode"].toStringRef());
+    out.resize(6);
+    return differentiable_once(std::move(out), "the gated scan");
+  }
+};
+
+// (y, final_state), differentiable in x, decay_logits and initial_state.
+std::tuple<torch::Tensor, torch::Tensor> pretrain_tmix_gated_scan(const torch::Tensor& x, const torch::Tensor& decay_logits,
+                                                                  const Optional& initial_state, const Optional& cu_seqlens,
+                                                                  const std::string& decay_mode, const std::string& input_mode) {
+  const bool differentiable = torch::GradMode::is_enabled() && (x.requires_grad() || decay_logits.requires_grad() ||
+                                                               (initial_state.has_value() && initial_state->requires_grad()));
+  if (!differentiable) {
+    const Forward f = train_forward(x, decay_logits, initial_state, cu_seqlens, decay_mode, input_mode);
+    return {f.y, f.final_state};
+  }
+  const auto out = TrainFunction::apply(x, decay_logits, initial_state, cu_seqlens, decay_mode, input_mode);
+  return {out[0], out[1]};
 }
 
 }  // namespace
@@ -191,11 +237,7 @@ void register_tmix_gated_scan_bindings(py::module_& module) {
              py::arg("query_start_loc"), py::arg("state_indices"), py::arg("state"), py::arg("x"),
              py::arg("decay_logits"), py::arg("decay_bias") = py::none(), py::arg("validated_metadata") = py::none(),
              py::arg("max_seqlen") = -1, py::arg("decay_mode") = "logits", py::arg("input_mode") = "unit");
-  module.def("pretrain_tmix_gated_scan_forward", &pretrain_tmix_gated_scan_forward, "Gated scan training forward",
-             py::arg("x"), py::arg("decay_logits"), py::arg("initial_state"), py::arg("cu_seqlens"),
-             py::arg("decay_mode"), py::arg("input_mode"));
-  module.def("pretrain_tmix_gated_scan_backward", &pretrain_tmix_gated_scan_backward, "Gated scan training backward",
-             py::arg("x"), py::arg("decay_logits"), py::arg("initial_state"), py::arg("query_start_loc"),
-             py::arg("status"), py::arg("boundary"), py::arg("grad_output"), py::arg("grad_final"),
-             py::arg("decay_mode"), py::arg("input_mode"));
+  module.def("pretrain_tmix_gated_scan", &pretrain_tmix_gated_scan, "Differentiable gated scan: (y, final_state)",
+             py::arg("x"), py::arg("decay_logits"), py::arg("initial_state") = py::none(), py::arg("cu_seqlens") = py::none(),
+             py::arg("decay_mode") = "logits", py::arg("input_mode") = "unit");
 }

@@ -58,8 +58,13 @@ RowsShape check_logits(const torch::Tensor& logits, const torch::Tensor& token_i
   return s;
 }
 
-py::tuple head_token_logprobs_forward(const torch::Tensor& logits, const torch::Tensor& token_ids, double temperature,
-                                      int64_t top_k, int64_t ignore_index) {
+struct Forward {
+  torch::Tensor logprobs, entropy, stats;
+  Optional top_ids, top_logprobs;
+};
+
+Forward rows_forward(const torch::Tensor& logits, const torch::Tensor& token_ids, double temperature, int64_t top_k,
+                     int64_t ignore_index) {
   need_value(top_k >= 0 && top_k <= FRWKV_TOP_K_MAX, "top_k must be in 0.." + std::to_string(FRWKV_TOP_K_MAX));
   const RowsShape s = check_logits(logits, token_ids, temperature);
   need_value(top_k <= s.vocab, "top_k must not exceed the vocabulary");
@@ -83,26 +88,17 @@ py::tuple head_token_logprobs_forward(const torch::Tensor& logits, const torch::
         stats.data_ptr<float>(), top_k > 0 ? top_ids->data_ptr<int64_t>() : nullptr,
         top_k > 0 ? top_logprobs->data_ptr<float>() : nullptr,
         at::cuda::getCurrentCUDAStream(logits.device().index()).stream()));
-  return py::make_tuple(logprobs, entropy, stats, top_ids, top_logprobs);
+  return Forward{logprobs, entropy, stats, top_ids, top_logprobs};
 }
 
-torch::Tensor head_token_logprobs_backward(const torch::Tensor& logits, const torch::Tensor& token_ids,
-                                           double temperature, int64_t ignore_index, const torch::Tensor& stats,
-                                           const torch::Tensor& entropy, const Optional& grad_logprobs,
-                                           const Optional& grad_entropy) {
+torch::Tensor rows_backward(const torch::Tensor& logits, const torch::Tensor& token_ids, double temperature, int64_t ignore_index,
+                            const torch::Tensor& stats, const torch::Tensor& entropy, const torch::Tensor& grad_logprobs,
+                            const torch::Tensor& grad_entropy) {
   const RowsShape s = check_logits(logits, token_ids, temperature);
-  need_value(stats.numel() == 2 * token_ids.numel() && entropy.numel() == token_ids.numel(),
-             "stats and entropy must be those of the forward call");
   const c10::cuda::CUDAGuard guard(logits.device());
   const auto ids = token_ids.contiguous();
-  const auto row_gradient = [&](const Optional& g, const char* name) {
-    if (!g.has_value()) return torch::Tensor();
-    need_type(g->scalar_type() == torch::kFloat32, std::string(name) + " must have dtype float32");
-    need_value(g->sizes() == token_ids.sizes() && g->device() == logits.device(),
-               std::string(name) + " must have one entry per row on the device of logits");
-    return g->contiguous();
-  };
-  const auto dlp = row_gradient(grad_logprobs, "grad_logprobs"), dent = row_gradient(grad_entropy, "grad_entropy");
+  const auto row_gradient = [](const torch::Tensor& g) { return g.defined() ? g.contiguous() : g; };
+  const auto dlp = row_gradient(grad_logprobs), dent = row_gradient(grad_entropy);
   auto dlogits = torch::empty(logits.sizes(), logits.options());
   if (token_ids.numel() > 0)
     check_abi(frwkv_sm100_token_logprobs_backward(
@@ -114,14 +110,47 @@ torch::Tensor head_token_logprobs_backward(const torch::Tensor& logits, const to
   return dlogits;
 }
 
+class RowsFunction : public torch::autograd::Function<RowsFunction> {
+ public:
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const torch::Tensor& logits,
+                                                const torch::Tensor& token_ids, double temperature, int64_t top_k,
+                                                int64_t ignore_index) {
+    const Forward f = rows_forward(logits, token_ids, temperature, top_k, ignore_index);
+    ctx->save_for_backward({logits, token_ids, f.stats, f.entropy});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->set_materialize_grads(false);
+    if (!f.top_ids.has_value()) return {f.logprobs, f.entropy};
+    ctx->mark_non_differentiable({*f.top_ids, *f.top_logprobs});
+    return {f.logprobs, f.entropy, *f.top_ids, *f.top_logprobs};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    torch::autograd::variable_list out{rows_backward(saved[0], saved[1], ctx->saved_data["temperature"].toDouble(),
+                                                     ctx->saved_data["ignore_index"].toInt(), saved[2], saved[3], grads[0], grads[1])};
+    out.resize(5);
+    return differentiable_once(std::move(out), "the token log probabilities operator");
+  }
+};
+
+// (logprobs, entropy, top_ids or None, top_logprobs or None), the first two differentiable in logits.
+std::tuple<torch::Tensor, torch::Tensor, Optional, Optional> head_token_logprobs(const torch::Tensor& logits,
+                                                                                 const torch::Tensor& token_ids, double temperature,
+                                                                                 int64_t top_k, int64_t ignore_index) {
+  if (!(torch::GradMode::is_enabled() && logits.requires_grad())) {
+    const Forward f = rows_forward(logits, token_ids, temperature, top_k, ignore_index);
+    return {f.logprobs, f.entropy, f.top_ids, f.top_logprobs};
+  }
+  const auto out = RowsFunction::apply(logits, token_ids, temperature, top_k, ignore_index);
+  const bool top = out.size() > 2;
+  return {out[0], out[1], top ? Optional(out[2]) : std::nullopt, top ? Optional(out[3]) : std::nullopt};
+}
+
 }  // namespace
 
 void register_rl_infctx_head_token_logprobs_bindings(py::module_& module) {
-  module.def("head_token_logprobs_forward", &head_token_logprobs_forward,
-             "Log probabilities of given tokens, entropy and top alternatives", py::arg("logits"), py::arg("token_ids"),
-             py::arg("temperature") = 1.0, py::arg("top_k") = 0, py::arg("ignore_index") = -100);
-  module.def("head_token_logprobs_backward", &head_token_logprobs_backward,
-             "Gradient of the token log probabilities and the entropy", py::arg("logits"), py::arg("token_ids"),
-             py::arg("temperature"), py::arg("ignore_index"), py::arg("stats"), py::arg("entropy"),
-             py::arg("grad_logprobs"), py::arg("grad_entropy"));
+  module.def("head_token_logprobs", &head_token_logprobs, "Log probabilities of given tokens, entropy and top alternatives",
+             py::arg("logits"), py::arg("token_ids"), py::arg("temperature") = 1.0, py::arg("top_k") = 0,
+             py::arg("ignore_index") = -100);
 }

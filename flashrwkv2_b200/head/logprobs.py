@@ -12,7 +12,6 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from ..tmix.wkv7 import _extension
 
@@ -22,26 +21,6 @@ class TokenLogprobs(NamedTuple):
     entropy: torch.Tensor              # float32, the shape of token_ids
     top_ids: torch.Tensor | None       # int64 [..., top_k], most probable first; None when top_k is 0
     top_logprobs: torch.Tensor | None  # float32 [..., top_k]
-
-
-class _TokenLogprobs(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, token_ids, temperature, top_k, ignore_index):
-        logprobs, entropy, stats, top_ids, top_logprobs = _extension().head_token_logprobs_forward(
-            logits, token_ids, temperature, top_k, ignore_index)
-        ctx.save_for_backward(logits, token_ids, stats, entropy)
-        ctx.settings = temperature, ignore_index
-        ctx.set_materialize_grads(False)
-        if top_k:
-            ctx.mark_non_differentiable(top_ids, top_logprobs)
-        return logprobs, entropy, top_ids, top_logprobs
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_logprobs, grad_entropy, _ids, _top):
-        logits, token_ids, stats, entropy = ctx.saved_tensors
-        return _extension().head_token_logprobs_backward(
-            logits, token_ids, *ctx.settings, stats, entropy, grad_logprobs, grad_entropy), None, None, None, None
 
 
 def rl_infctx_head_token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor, *, temperature: float = 1.0,
@@ -57,11 +36,7 @@ def rl_infctx_head_token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
     logprob is -inf, entropy and gradient are 0.  A NaN or +inf makes its row's results NaN.
 
     Errors: ``TypeError`` for wrong types, ``ValueError`` for wrong shapes, layouts and values, before any launch."""
-    if isinstance(logits, torch.Tensor) and logits.requires_grad and torch.is_grad_enabled():
-        return TokenLogprobs(*_TokenLogprobs.apply(logits, token_ids, temperature, top_k, ignore_index))
-    logprobs, entropy, _, top_ids, top_logprobs = _extension().head_token_logprobs_forward(
-        logits, token_ids, temperature, top_k, ignore_index)
-    return TokenLogprobs(logprobs, entropy, top_ids, top_logprobs)
+    return TokenLogprobs(*_extension().head_token_logprobs(logits, token_ids, temperature, top_k, ignore_index))
 
 
 __all__ = ["TokenLogprobs", "rl_infctx_head_token_logprobs"]

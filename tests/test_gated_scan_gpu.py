@@ -476,3 +476,28 @@ def test_training_changed_input_is_noticed():
     x.add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_training_is_differentiable_once():
+    from flashrwkv2_b200 import pretrain_tmix_gated_scan_fp32io16 as op
+
+    x, decay = (torch.randn(1, 10, 8, device=DEV, requires_grad=True) for _ in range(2))
+    y, _ = op(x, decay)
+    plain, = torch.autograd.grad(y.sum(), x, retain_graph=True)
+    recorded, = torch.autograd.grad(y.sum(), x, create_graph=True)
+    assert torch.equal(plain, recorded)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        recorded.sum().backward()
+
+
+def test_training_without_gradients_builds_no_graph():
+    from flashrwkv2_b200 import pretrain_tmix_gated_scan_fp32io16 as op
+
+    x, decay = (torch.randn(1, 10, 8, device=DEV, requires_grad=True) for _ in range(2))
+    with torch.no_grad():
+        y, final = op(x, decay)
+    assert not y.requires_grad and not final.requires_grad
+    y, final = op(x.detach(), decay.detach())
+    assert not y.requires_grad and not final.requires_grad
+    y, final = op(x.detach(), decay)  # one input alone
+    assert torch.autograd.grad(y.sum() + final.sum(), decay)[0].shape == decay.shape

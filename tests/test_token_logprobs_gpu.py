@@ -374,3 +374,23 @@ def test_rollouts_through_scan_head_and_loss():
     for k in leaves:
         top = float(cpu[k].grad.abs().max())
         assert float((gpu[k].grad.cpu().double() - cpu[k].grad).abs().max()) <= 2.0 ** -14 * top, k
+
+
+def test_differentiable_once_and_no_graph_without_need():
+    from flashrwkv2_b200 import rl_infctx_head_token_logprobs as op
+
+    logits, ids, a, b = case(3, 40, torch.float32, seed=15)
+    x, ids = logits.to(DEV).requires_grad_(), ids.to(DEV)
+    out = op(x, ids, top_k=2)
+    assert out.logprobs.requires_grad and out.entropy.requires_grad and not out.top_logprobs.requires_grad
+    recorded, = torch.autograd.grad(out.logprobs.sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        recorded.sum().backward()
+    with torch.no_grad():
+        assert not op(x, ids).logprobs.requires_grad
+    assert not op(x.detach(), ids).logprobs.requires_grad
+    out = op(x, ids)
+    with torch.no_grad():
+        x.add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.logprobs.sum().backward()
