@@ -127,21 +127,21 @@ template <typename io_t, bool ALIGNED, int S> struct Rows {
   // A lane's 8 bytes of the rows of a group; `from` is the global address of its first row's 64 bytes.
   struct Mine {
     const uint2 *even, *odd;  // ALIGNED
-    unsigned space, first, step;
+    // Otherwise where row i's bytes begin, less i rows: the shift repeats every kPeriod rows.  16-bit types read the words that
+    // hold them and shift by the rest.
+    static constexpr int kPeriod = ALIGNED ? 1 : 16 / static_cast<int>(sizeof(io_t));
+    unsigned at[kPeriod], shift[2];
 
     __device__ __forceinline__ Lanes<V> operator[](int i) const {
       if constexpr (ALIGNED) {
         return unpack<io_t>((i & 1 ? odd : even)[i * kLanes]);
       } else {
-        const unsigned at = space + i * kPitch + ((first + i * step) & 15u);
-        const unsigned word = sizeof(io_t) == 4 ? at : at & ~3u;
         unsigned w[3] = {0, 0, 0};
 #pragma unroll
         for (int k = 0; k < (sizeof(io_t) == 4 ? 2 : 3); ++k)
-          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[k]) : "r"(word + 4 * k) : "memory");
+          asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[k]) : "r"(at[i % kPeriod] + i * kPitch + 4 * k) : "memory");
         if constexpr (sizeof(io_t) == 4) return unpack<io_t>(make_uint2(w[0], w[1]));
-        const unsigned shift = (at & 2u) * 8u;
-        return unpack<io_t>(make_uint2(__funnelshift_r(w[0], w[1], shift), __funnelshift_r(w[1], w[2], shift)));
+        return unpack<io_t>(make_uint2(__funnelshift_r(w[0], w[1], shift[i & 1]), __funnelshift_r(w[1], w[2], shift[i & 1])));
       }
     }
   };
@@ -153,9 +153,13 @@ template <typename io_t, bool ALIGNED, int S> struct Rows {
       m.even = at + static_cast<int>(threadIdx.x) % kLanes + swap;
       m.odd = m.even - 2 * swap;
     } else {
-      m.space = static_cast<unsigned>(__cvta_generic_to_shared(at)) + threadIdx.x % kLanes * 8;
-      m.first = static_cast<unsigned>(reinterpret_cast<uintptr_t>(from));
-      m.step = static_cast<unsigned>(stride) * static_cast<unsigned>(sizeof(io_t));
+      const unsigned start = static_cast<unsigned>(__cvta_generic_to_shared(at)) + threadIdx.x % kLanes * 8;
+      const unsigned first = static_cast<unsigned>(reinterpret_cast<uintptr_t>(from));
+      const unsigned step = static_cast<unsigned>(stride) * static_cast<unsigned>(sizeof(io_t));
+#pragma unroll
+      for (int k = 0; k < Mine::kPeriod; ++k) m.at[k] = (start + ((first + k * step) & 15u)) & ~3u;
+      m.shift[0] = (first & 2u) * 8u;
+      m.shift[1] = ((first + step) & 2u) * 8u;
     }
     return m;
   }
