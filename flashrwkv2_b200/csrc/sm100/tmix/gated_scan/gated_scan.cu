@@ -302,6 +302,10 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_fo
 // state pool is most of what a step reads and writes.
 template <typename io_t, int V, bool LOGITS, bool COMPLEMENT>
 __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanParams p) {
+  // The next step's launch may begin while this one runs, and this one may have begun while the launch before it ran
+  // (programmatic dependent launch); nothing is read before that one is done.
+  asm volatile("griddepcontrol.launch_dependents;" : : : "memory");
+  asm volatile("griddepcontrol.wait;" : : : "memory");
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, nullptr, 0);
     return;
@@ -648,7 +652,16 @@ int run_steps(const GatedScanParams& p, int io_dtype, int decay_mode, int input_
   const unsigned grid = static_cast<unsigned>((static_cast<long long>(p.n_seq) * (p.channels / (vectors ? wide : 1)) + 255) / 256);
   with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
     const auto launch = [&](auto io, auto v) {
-      gated_scan_step_kernel<decltype(io), v(), logits(), complement()><<<grid, 256, 0, s>>>(p);
+      cudaLaunchAttribute dependent;
+      dependent.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      dependent.val.programmaticStreamSerializationAllowed = 1;
+      cudaLaunchConfig_t config = {};
+      config.gridDim = dim3(grid);
+      config.blockDim = dim3(256);
+      config.stream = s;
+      config.attrs = &dependent;
+      config.numAttrs = 1;
+      cudaLaunchKernelEx(&config, gated_scan_step_kernel<decltype(io), v(), logits(), complement()>, p);
     };
     using one = std::integral_constant<int, 1>;
     if (io_dtype == FRWKV_IO_FP32) vectors ? launch(float{}, std::integral_constant<int, 4>{}) : launch(float{}, one{});
