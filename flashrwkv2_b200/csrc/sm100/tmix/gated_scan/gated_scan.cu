@@ -179,6 +179,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_fo
   Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, n_seq, lengths);
   const int channel = unit.channel, count = min(V, p.channels - channel);
   const int block_channel = channel - lane % kLanes * V, block_count = min(kLanes * V, p.channels - block_channel);
+  const long long least_stride = min(p.x_stride, p.decay_stride);
   const auto first_tile = [&](int seq) {
     if (seq < 0) return Tile{-1, 0, 0, 0};
     const int begin = row_begin(p, seq);
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_fo
     return at - rank * kTile < t.len ? Tile{t.seq, t.begin, at, t.len} : first_tile(unit.next());
   };
   const auto is_full = [&](const Tile& t) {
-    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || t.begin + t.at > 0);
+    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || (t.begin + t.at) * least_stride >= 16);
   };
   const int warp_row = warp * kGroups * S, own = warp_row + lane / kLanes * S;  // first rows in a tile
   uint2* const decays = staged + (2 * kWarps + warp) * R::kWords;
@@ -395,6 +396,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   Unit unit = unit_of<V>(p, grid, static_cast<int>(blockIdx.x) / ranks, p.n_seq, lengths);
   const int channel = unit.channel, count = min(V, p.channels - channel);
   const int block_channel = channel - lane % kLanes * V, block_count = min(kLanes * V, p.channels - block_channel);
+  const long long least_stride = min(p.x_stride, p.decay_stride);
   const int step_rows = ranks * kTile;
   const auto first_tile = [&](int seq) {
     if (seq < 0) return Tile{-1, 0, 0, 0};
@@ -405,7 +407,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     return t.at >= step_rows ? Tile{t.seq, t.begin, t.at - step_rows, t.len} : first_tile(unit.next());
   };
   const auto is_full = [&](const Tile& t) {
-    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || t.begin + t.at > 0);
+    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || (t.begin + t.at) * least_stride >= 16);
   };
   // In memory the lane groups of a warp lie as in the forward pass, first in time first; along the chain a lane works on
   // group kGroups - 1 - lane / kLanes.

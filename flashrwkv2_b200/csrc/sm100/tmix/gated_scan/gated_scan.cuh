@@ -182,7 +182,7 @@ template <typename io_t, bool ALIGNED, int S> struct Rows {
     }
   }
   // Rows [0, rows) of `base` + row * stride (for this warp), `channels` of the block's 8 * V; what does not exist is not read.
-  // FULL: all of them exist, and the tensor's first row is not among them.  `tensor` is its first element.
+  // FULL: all of them exist and lie 16 bytes or more behind the tensor's beginning.  `tensor` is its first element.
   template <bool FULL>
   static __device__ __forceinline__ void fetch(uint2* space, const io_t* base, long long stride, int rows, int channels, const io_t* tensor) {
     const int lane = threadIdx.x & 31;

@@ -249,7 +249,8 @@ int frwkv_sm100_wkv7_pretrain_backward(const void* r, const void* w, const void*
  *   y          : [total_tokens, channels], contiguous, token dtype;
  *   cu_seqlens, slots, status, max_seqlen : as in frwkv_sm100_wkv7_recurrent, with the same fail-closed rules
  *                (invalid metadata: y NaN-filled, pool untouched; rows behind the last active sequence untouched);
- * Any number of channels; channels, strides and starts that are multiples of 8 bytes run fastest. */
+ * Any number of channels and any alignment of the element; channels, strides and starts that are multiples of 16 bytes
+ * run fastest. */
 int frwkv_sm100_gated_scan(
     const int32_t* cu_seqlens, const int32_t* slots, const int32_t* status, float* state_pool, const void* x,
     long long x_row_stride, const void* decay, long long decay_row_stride, const void* decay_bias, void* y, int n_seq,

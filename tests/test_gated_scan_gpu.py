@@ -135,6 +135,51 @@ def test_rows_of_a_wider_projection(dtype, offset, width):
     check_serve(c, y.cpu(), pool.cpu(), "logits", "unit")
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_row_for_all_tokens(dtype):
+    """Rows at distance 0 (an expanded tensor), from a start that is aligned to the element only."""
+    from flashrwkv2_b200 import infer_tmix_gated_scan_fp32io16_forward_varlen as op
+
+    c = case([300, 290], 70, dtype, "logits", seed=16)
+    row = torch.full((73,), math.nan, dtype=dtype)
+    row[1:71] = c["x"][0]
+    c["x"] = c["x"][:1].expand(590, 70).contiguous()
+    x = row.to(DEV)[1:71].expand(590, 70)
+    assert x.stride(0) == 0
+    pool = c["pool"].to(DEV)
+    y = op(x, c["decay"].to(DEV), state_pool=pool, cu_seqlens=c["cu"].to(DEV), state_indices=c["slots"].to(DEV))
+    check_serve(c, y.cpu(), pool.cpu(), "logits", "unit")
+
+
+def test_very_many_sequences():
+    """Several sequences to a unit of work; short ones, which the step kernel serves, among them."""
+    g = torch.Generator().manual_seed(5)
+    c = case(torch.randint(1, 33, (1100,), generator=g).tolist(), 992, torch.bfloat16, "logits", seed=17)
+    y, pool = serve(c, "logits", "unit")
+    check_serve(c, y, pool, "logits", "unit")
+    c, initial, dy, dfinal = train_case(torch.randint(1, 20, (1100,), generator=g).tolist(), 992, torch.bfloat16, "logits", 18)
+    got = train(c["x"], c["decay"], initial, dy, dfinal, "logits", "unit", cu=c["cu"])
+    check_train(c, got, initial, dy, dfinal, "logits", "unit")
+
+
+def test_offsets_beyond_two_to_the_thirty_one_elements():
+    """66000 rows of 32800 channels: the last rows lie past 2^31 elements.  Channels are independent, so the last eight of them
+    against the oracle say whether every offset is right."""
+    from flashrwkv2_b200 import infer_tmix_gated_scan_fp32io16_forward_varlen as op
+
+    rows, channels = 66000, 32800
+    if torch.cuda.mem_get_info()[0] < 24 << 30:
+        pytest.skip("needs 24 GB")
+    small = case([rows - 3000, 3000], 8, torch.bfloat16, "retention", seed=19, spare=0)
+    x, decay = (torch.zeros(rows, channels, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    x[:, -8:], decay[:, -8:] = small["x"].to(DEV), small["decay"].to(DEV)
+    pool = torch.zeros(2, channels, device=DEV)
+    pool[:, -8:] = small["pool"].to(DEV)
+    y = op(x, decay, state_pool=pool, cu_seqlens=small["cu"].to(DEV), state_indices=small["slots"].to(DEV), decay_mode="retention")
+    check_serve(small, y[:, -8:].cpu(), pool[:, -8:].cpu(), "retention", "unit")
+    assert float(y[:, :-8].abs().max()) == 0 and float(pool[:, :-8].abs().max()) == 0
+
+
 def test_extreme_logits_and_retentions():
     big = torch.tensor([-math.inf, -200.0, -90.0, -30.0, -17.0, 17.0, 30.0, 100.0, math.inf, 0.0])
     c = case([50], 10, torch.float32, "logits", seed=10)
