@@ -21,8 +21,9 @@ namespace cg = cooperative_groups;
 constexpr int kTile = 256;           // tokens of a CTA's tile
 constexpr int S = 16;                // tokens of a lane in a tile
 constexpr int kWarps = kTile / (kGroups * S), kThreads = kWarps * 32;
-// CTAs per SM, by registers and by the staging of their rows
-constexpr int forward_ctas(bool aligned) { return aligned ? 4 : 3; }
+// CTAs per SM, by registers and by the staging of their rows.  Copies of 4 bytes go through L1, which the staging of a fourth
+// CTA would leave too small (16 x 1024 rows of 1003 fp32 channels: 86 us with four, 56 us with three).
+constexpr int forward_ctas(int align) { return align == 16 ? 4 : 3; }
 constexpr int kBackwardCtas = 2;
 constexpr int kMaxCluster = 8;
 constexpr int kShortRows = 16;       // sequences of at most this many tokens are served by the step kernel
@@ -159,12 +160,12 @@ __device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Pieces<V>* s
 
 // ---- forward
 
-template <typename io_t, bool ALIGNED, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
+template <typename io_t, int ALIGN, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
+__global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
-  using R = Rows<io_t, ALIGNED, S>;
+  using R = Rows<io_t, ALIGN, S>;
   extern __shared__ uint2 staged[];  // x of two tiles, then the decays of one: [warp][R::kWords]
   __shared__ int lengths[kRanked];
   __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_fo
     return at - rank * kTile < t.len ? Tile{t.seq, t.begin, at, t.len} : first_tile(unit.next());
   };
   const auto is_full = [&](const Tile& t) {
-    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || (t.begin + t.at) * least_stride >= 16);
+    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGN != 0 || (t.begin + t.at) * least_stride >= 16);
   };
   const int warp_row = warp * kGroups * S, own = warp_row + lane / kLanes * S;  // first rows in a tile
   uint2* const decays = staged + (2 * kWarps + warp) * R::kWords;
@@ -270,7 +271,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGNED)) gated_scan_fo
     const int left = tile.len - tile.at - own;
     if (p.boundary != nullptr && left > 0) {
       float* to = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;
-      if (ALIGNED && count == V) store_states_whole<V>(to, h);
+      if (ALIGN == 16 && count == V) store_states_whole<V>(to, h);
       else store_states<V>(to, h, count);
     }
     if (next.seq != tile.seq) carry = initial_state(next);
@@ -376,13 +377,13 @@ __global__ void __launch_bounds__(256) gated_scan_step_kernel(const GatedScanPar
 // tiles; inside a tile warps, lane groups and rows are counted from its end, so that all joins are those of the forward
 // pass.  The states come from those that the forward pass saved before every lane's rows.
 
-template <typename io_t, bool ALIGNED, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
+template <typename io_t, int ALIGN, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
 __global__ void __launch_bounds__(kThreads, kBackwardCtas)
 gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t), kWarpRows = kGroups * S;
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
-  using R = Rows<io_t, ALIGNED, S>;
+  using R = Rows<io_t, ALIGN, S>;
   extern __shared__ uint2 staged[];  // x and the decays of one tile, then dy of two: [warp][R::kWords]
   __shared__ int lengths[kRanked];
   __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
@@ -407,7 +408,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     return t.at >= step_rows ? Tile{t.seq, t.begin, t.at - step_rows, t.len} : first_tile(unit.next());
   };
   const auto is_full = [&](const Tile& t) {
-    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGNED || (t.begin + t.at) * least_stride >= 16);
+    return t.at + kTile <= t.len && block_count == kLanes * V && (ALIGN != 0 || (t.begin + t.at) * least_stride >= 16);
   };
   // In memory the lane groups of a warp lie as in the forward pass, first in time first; along the chain a lane works on
   // group kGroups - 1 - lane / kLanes.
@@ -444,7 +445,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     L h = L::all(0.0f);
     if (left > 0) {
       const float* from = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;
-      h = ALIGNED && count == V ? load_states_whole<V>(from) : load_states<V>(from, count);
+      h = ALIGN == 16 && count == V ? load_states_whole<V>(from) : load_states<V>(from, count);
     }
     copies_done();
     __syncwarp();  // what the warp's other lanes copied
@@ -572,18 +573,28 @@ template <typename F> void with_modes(int decay_mode, int input_mode, F f) {
   }
 }
 
-// Calls f with the token type, and whether all rows begin at multiples of 16 bytes, as compile-time constants.
-template <typename F> void with_type(int io_dtype, bool aligned, F f) {
-  using yes = std::true_type;
-  using no = std::false_type;
-  if (io_dtype == FRWKV_IO_FP32) aligned ? f(float{}, yes{}) : f(float{}, no{});
-  else if (io_dtype == FRWKV_IO_BF16) aligned ? f(__nv_bfloat16{}, yes{}) : f(__nv_bfloat16{}, no{});
-  else aligned ? f(__half{}, yes{}) : f(__half{}, no{});
+// Calls f with the token type and the rows' alignment as compile-time constants.
+template <typename F> void with_type(int io_dtype, int align, F f) {
+  using none = std::integral_constant<int, 0>;
+  using four = std::integral_constant<int, 4>;
+  using all = std::integral_constant<int, 16>;
+  const auto with_align = [&](auto io) {
+    if (align == 16) f(io, all{});
+    else if (align == 4) f(io, four{});
+    else f(io, none{});
+  };
+  if (io_dtype == FRWKV_IO_FP32) with_align(float{});
+  else if (io_dtype == FRWKV_IO_BF16) with_align(__nv_bfloat16{});
+  else with_align(__half{});
 }
 
-bool rows_aligned(const GatedScanParams& p, int io_dtype, std::initializer_list<const void*> rows) {
-  const int n = io_dtype == FRWKV_IO_FP32 ? 4 : 8;
-  return p.channels % n == 0 && p.x_stride % n == 0 && p.decay_stride % n == 0 && multiple_of(16, rows);
+// 16 or 4 where the channels, the strides and all starts are multiples of that many bytes, else 0.
+int alignment_of(const GatedScanParams& p, int io_dtype, std::initializer_list<const void*> rows) {
+  for (int align : {16, 4}) {
+    const int n = align / (io_dtype == FRWKV_IO_FP32 ? 4 : 2);
+    if (p.channels % n == 0 && p.x_stride % n == 0 && p.decay_stride % n == 0 && multiple_of(align, rows)) return align;
+  }
+  return 0;
 }
 
 // How the work is cut.  Few sequences with few channels leave the GPU empty, so a cluster shares a sequence: the size that
@@ -633,14 +644,14 @@ int launch(K kernel, const Grid& g, const GatedScanParams& p, int words, void* s
 
 int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int input_mode, int max_seqlen, void* stream) {
   int rc = FRWKV_OK;
-  with_type(io_dtype, rows_aligned(p, io_dtype, {p.x, p.decay, p.y, p.boundary}), [&](auto io, auto aligned) {
+  with_type(io_dtype, alignment_of(p, io_dtype, {p.x, p.decay, p.y, p.boundary}), [&](auto io, auto align) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
-      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(aligned()) * sm_count());
-      constexpr int kWords = 3 * Rows<io_t, aligned(), S>::kWords;
+      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(align()) * sm_count());
+      constexpr int kWords = 3 * Rows<io_t, align(), S>::kWords;
       constexpr const char* kName = "gated_scan_forward_kernel";
-      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, aligned(), logits(), complement(), true>, g, p, kWords, stream, kName)
-                         : launch(gated_scan_forward_kernel<io_t, aligned(), logits(), complement(), false>, g, p, kWords, stream, kName);
+      rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, align(), logits(), complement(), true>, g, p, kWords, stream, kName)
+                         : launch(gated_scan_forward_kernel<io_t, align(), logits(), complement(), false>, g, p, kWords, stream, kName);
     });
   });
   return rc;
@@ -734,14 +745,15 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
                           total_tokens / n_seq, 0};
   const GatedScanGrads g{dy, dfinal, dx, ddecay, dinitial};
   int rc = FRWKV_OK;
-  with_type(io_dtype, rows_aligned(p, io_dtype, {x, decay, dy, dx, ddecay, boundary}), [&](auto io, auto aligned) {
+  with_type(io_dtype, alignment_of(p, io_dtype, {x, decay, dy, dx, ddecay, boundary}) == 16 ? 16 : 0, [&](auto io, auto alignment) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
+      constexpr int kAlign = alignment() == 16 ? 16 : 0;  // by pieces rather than by 4 bytes
       const Grid grid = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), kBackwardCtas * sm_count());
-      constexpr int kWords = 4 * Rows<io_t, aligned(), S>::kWords;
+      constexpr int kWords = 4 * Rows<io_t, kAlign, S>::kWords;
       constexpr const char* kName = "gated_scan_backward_kernel";
-      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, aligned(), logits(), complement(), true>, grid, p, kWords, stream, kName, g)
-                            : launch(gated_scan_backward_kernel<io_t, aligned(), logits(), complement(), false>, grid, p, kWords, stream, kName, g);
+      rc = grid.cluster > 1 ? launch(gated_scan_backward_kernel<io_t, kAlign, logits(), complement(), true>, grid, p, kWords, stream, kName, g)
+                            : launch(gated_scan_backward_kernel<io_t, kAlign, logits(), complement(), false>, grid, p, kWords, stream, kName, g);
     });
   });
   return rc;

@@ -109,14 +109,17 @@ template <typename io_t> __device__ __forceinline__ uint2 pack(const Lanes<8 / s
 
 // ---- token rows in shared memory
 //
-// A warp's rows of one tensor: four lane groups of S rows of 64 bytes each.  ALIGNED: every row's 64 bytes begin at a multiple
-// of 16 in global memory.  Otherwise the five 16-byte pieces that a row's 64 bytes touch are copied, as far as they hold bytes
-// of the row or of what lies before it in the tensor, and a lane shifts its 8 bytes out of them: four times fewer accesses
-// than element by element (16 x 1024 rows of 1003 fp32 channels).
+// A warp's rows of one tensor: four lane groups of S rows of 64 bytes each.  ALIGN is what every row's 64 bytes begin at a
+// multiple of in global memory: 16, 4, or nothing in particular (0).  With 16 they are copied by 16 bytes, with 4 by 4.
+// Otherwise the five 16-byte pieces that a row's 64 bytes touch are copied, as far as they hold bytes of the row or of what
+// lies before it in the tensor, and a lane shifts its 8 bytes out of them.  (16 x 1024 rows of 1003 fp32 channels, by 4 bytes
+// and by pieces: forward 57 and 67 us, backward 150 and 106 us.  32 x 1024 rows of 1003 bf16 channels, element by element
+// and by pieces: 290 and 88 us, 589 and 146 us.)
 
 constexpr int kLanes = 8, kGroups = 32 / kLanes;  // lanes along the channels (8 bytes each), groups of them along time
 
-template <typename io_t, bool ALIGNED, int S> struct Rows {
+template <typename io_t, int ALIGN, int S> struct Rows {
+  static constexpr bool ALIGNED = ALIGN >= 4;  // as it lies in shared memory
   static constexpr int V = 8 / sizeof(io_t);
   static constexpr int kPitch = ALIGNED ? 64 : 80;  // bytes of a row
   // of a group, in words of 8 bytes.  Two groups that read their i-th rows at once have to read different banks: groups are an
@@ -190,20 +193,21 @@ template <typename io_t, bool ALIGNED, int S> struct Rows {
     const unsigned to = static_cast<unsigned>(__cvta_generic_to_shared(space));
     static_assert(S % 8 == 0, "eight rows at once are of one group");
     if constexpr (ALIGNED) {
-      constexpr int kElements = 16 / sizeof(io_t);
-      const io_t* from = base + first * stride + part * kElements;
-      const bool in = part * kElements < channels;
+      // kParts accesses a row, kAtOnce rows at once, which are of one group and whole pairs
+      constexpr int kElements = ALIGN / static_cast<int>(sizeof(io_t)), kParts = 64 / ALIGN, kAtOnce = 32 / kParts;
+      const int access = lane % kParts, at_once = lane / kParts;
+      const io_t* from = base + at_once * stride + access * kElements;
+      const bool in = access * kElements < channels;
 #pragma unroll
-      for (int i = 0; i < kGroups * S / 8; ++i) {
-        const int group = i * 8 / S;
-        const unsigned at = to + group * kGroupWords * 8 + (i * 8 - group * S) * 64 + (first ^ (group & 1)) * 64 + part * 16;
-        if constexpr (FULL) {
-          copy(at, from, 16);
-        } else {
-          const bool there = in && i * 8 + first < rows;
+      for (int i = 0; i < kGroups * S / kAtOnce; ++i) {
+        const int group = i * kAtOnce / S;
+        const unsigned at = to + group * kGroupWords * 8 + (i * kAtOnce - group * S) * 64 + (at_once ^ (group & 1)) * 64 + access * ALIGN;
+        const bool there = FULL || (in && i * kAtOnce + at_once < rows);
+        if constexpr (ALIGN == 16)
           copy(at, there ? from : tensor, there ? 16 : 0);
-        }
-        from += 8 * stride;
+        else
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" : : "r"(at), "l"(there ? from : tensor), "r"(there ? 4 : 0) : "memory");
+        from += kAtOnce * stride;
       }
     } else {
       if constexpr (FULL) {
@@ -240,7 +244,7 @@ template <typename io_t, bool ALIGNED, int S> struct Rows {
   }
   template <bool FULL> static __device__ __forceinline__ void store(io_t* to, const Lanes<V>& a, int count) {
     const uint2 w = pack<io_t>(a);
-    if constexpr (ALIGNED) {
+    if constexpr (ALIGN == 16) {
       if (FULL || count > 0) __stcs(reinterpret_cast<uint2*>(to), w);
     } else if (FULL || count >= V) {
       if (sizeof(io_t) == 4 || (reinterpret_cast<uintptr_t>(to) & 2) == 0) {
