@@ -40,8 +40,12 @@ struct Rows {
   float inv_temperature;
 };
 
+// A row's first logit; rows and p.inner fit in 31 bits.
 template <typename io_t> __device__ __forceinline__ const io_t* row_start(const Rows& p, long long row) {
-  return static_cast<const io_t*>(p.logits) + row / p.inner * p.stride_outer + row % p.inner * p.stride_inner;
+  const unsigned at = static_cast<unsigned>(row), inner = static_cast<unsigned>(p.inner);
+  const unsigned outer = at < inner ? 0 : at / inner;
+  return static_cast<const io_t*>(p.logits) + static_cast<long long>(outer) * p.stride_outer +
+         static_cast<long long>(at - outer * inner) * p.stride_inner;
 }
 
 __device__ __forceinline__ long long row_id(const Rows& p, long long row) {
@@ -415,7 +419,7 @@ token_logprobs_kernel(const Rows p, int top_k, float* __restrict__ logprobs, flo
   __shared__ std::conditional_t<TOP, TopScratch, char> top_scratch[1];
   const cg::cluster_group cluster = cg::this_cluster();
   const int parts = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
-  const long long row = blockIdx.x / parts;
+  const long long row = blockIdx.x / static_cast<unsigned>(parts);
   const int tid = threadIdx.x;
   const long long id = row_id(p, row);
   if (id == p.ignore_index) {  // the whole cluster leaves
@@ -536,8 +540,9 @@ token_logprobs_backward_kernel(const Rows p, int segments, const float* __restri
                                const float* __restrict__ dlogprobs, const float* __restrict__ dentropy,
                                io_t* __restrict__ dlogits) {
   constexpr int kCount = Pack<io_t>::kCount;
-  const long long row = blockIdx.x / segments;
-  const int segment = static_cast<int>(blockIdx.x % segments), tid = threadIdx.x;
+  const unsigned row_index = blockIdx.x / static_cast<unsigned>(segments);
+  const long long row = row_index;
+  const int segment = static_cast<int>(blockIdx.x - row_index * segments), tid = threadIdx.x;
   const long long id = row_id(p, row);
   const io_t* x = row_start<io_t>(p, row);
   io_t* out = dlogits + row * p.vocab;
@@ -572,18 +577,22 @@ token_logprobs_backward_kernel(const Rows p, int segments, const float* __restri
     }
   }
   const int first = segment * kBatch * kThreads + tid;
+  x += lead + static_cast<long long>(first) * kCount;
+  out += lead + static_cast<long long>(first) * kCount;
+  // the given token's place, counted from this thread's first logit (far away where it is not among the row's packs)
+  const long long from_first = id - lead - static_cast<long long>(first) * kCount;
+  const int hit = from_first >= 0 && from_first < kBatch * kThreads * kCount ? static_cast<int>(from_first) : -1;
+  const int left = packs - first;
   Pack<io_t> v[kBatch];
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    if (!zero && first + i * kThreads < packs) v[i].load(x + lead + static_cast<long long>(first + i * kThreads) * kCount);
+    if (!zero && i * kThreads < left) v[i].load(x + i * kThreads * kCount);
     else v[i].raw = make_uint4(0, 0, 0, 0);
   }
   const float2 minus_m = make_float2(-m, -m), k2 = make_float2(k, k), c1_2 = make_float2(c1, c1), c0_2 = make_float2(c0, c0);
 #pragma unroll
   for (int i = 0; i < kBatch; ++i) {
-    const int pack = first + i * kThreads;
-    if (pack >= packs) break;
-    const int base = lead + pack * kCount;
+    if (i * kThreads >= left) break;
     unsigned words[4] = {0, 0, 0, 0};
     if (!zero) {
       float g[kCount];
@@ -595,10 +604,10 @@ token_logprobs_backward_kernel(const Rows p, int segments, const float* __restri
         g[2 * j] = y.x;
         g[2 * j + 1] = y.y;
       }
-      const long long hit = id - base;
-      if (hit >= 0 && hit < kCount) {
+      const unsigned place = static_cast<unsigned>(hit - i * kThreads * kCount);
+      if (place < kCount) {
 #pragma unroll
-        for (int j = 0; j < kCount; ++j) g[j] = j == hit ? g[j] + at_id : g[j];
+        for (int j = 0; j < kCount; ++j) g[j] = j == static_cast<int>(place) ? g[j] + at_id : g[j];
       }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -606,7 +615,7 @@ token_logprobs_backward_kernel(const Rows p, int segments, const float* __restri
         else words[j] = pack_two<io_t>(g[2 * j], g[2 * j + 1]);
       }
     }
-    __stcs(reinterpret_cast<uint4*>(out + base), make_uint4(words[0], words[1], words[2], words[3]));
+    __stcs(reinterpret_cast<uint4*>(out + i * kThreads * kCount), make_uint4(words[0], words[1], words[2], words[3]));
   }
 }
 
