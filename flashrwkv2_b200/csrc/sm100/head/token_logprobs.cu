@@ -6,7 +6,11 @@
 // Differences to m are formed before anything is scaled, so a common offset of a row costs no precision; exponents are
 // base 2 inside (z times log2 e).  Everything is fp32 but the logits and their gradient.
 //
-// Both directions are bound by HBM: the row is read once (backward: read once, written once).
+// The row is read once (backward: read once, written once), so HBM is the floor; an element also costs one exponential on the
+// SFU, 16 a clock and SM, which is 0.7 of that floor for 16-bit logits.  Measured on bf16: 4096 x 65536 91 us = 0.90 of the
+// HBM copy rate (106 us when it runs for seconds and the power limit takes the clock down), with the top 20 119 us;
+// 777 x 50277 fp32 28 us = 0.85 (777 CTAs are one round on 888 places); gradient of 2048 x 65536 84 us = 0.97.
+// 32 x 65536 with the top 20: 12.3 us, all latency (launch, load, selection, two cluster barriers).
 #include "../common.cuh"
 
 #include <cooperative_groups.h>
