@@ -33,8 +33,8 @@ def infer_tmix_gated_scan_fp32io16_forward_varlen(
     ``state_pool`` float32 ``[slots, C]``, ``decay_bias`` ``[C]`` (logits mode only).  Metadata, tickets, CUDA-graph use and
     the fail-closed rules are those of the WKV7 operators: without ``validated_metadata`` the metadata is checked on the
     host (one sync); with a capacity ticket nothing synchronises, rows behind the last active sequence are left as they
-    were allocated, and invalid metadata fills y with NaN and leaves the pool untouched.  A call needs its scratch to
-    itself until it has finished, which torch's allocator sees to; captured graphs own theirs."""
+    were allocated, and invalid metadata fills y with NaN and leaves the pool untouched.  No gradients: for those there is
+    the training form."""
     native = _extension()
     if validated_metadata is None and isinstance(x, torch.Tensor) and isinstance(state_pool, torch.Tensor) and x.is_cuda:
         validated_metadata = prepare_tmix_wkv7_recurrent_metadata(

@@ -16,8 +16,10 @@ def pretrain_tmix_gated_scan_fp32io16(
     ``x`` and ``decay_logits`` are dense ``[B, T, C]``, or packed ``[total_tokens, C]`` with ``cu_seqlens`` (int32 ``[N+1]``,
     non-empty sequences).  ``initial_state`` is float32 ``[B or N, C]`` (zeros when None), ``final_state`` the same shape.
     Gradients reach ``x``, ``decay_logits`` (the retention in that mode) and ``initial_state``, through y and through the
-    final state.  ``cu_seqlens`` is validated on the device without a sync: bad bounds make every output NaN.  The backward
-    pass can be captured into a CUDA graph together with its forward pass; it is differentiable once."""
+    final state.  Rows may lie apart (a slice of a wider projection) at one regular distance.  ``cu_seqlens`` is validated
+    on the device without a sync: bad bounds make every output NaN.  The backward pass can be captured into a CUDA graph
+    together with its forward pass, as torch asks for it: after a warm-up on a side stream, and with no other autograd
+    graph of the same leaves alive.  It is differentiable once."""
     return _extension().pretrain_tmix_gated_scan(x, decay_logits, initial_state, cu_seqlens, decay_mode, input_mode)
 
 
