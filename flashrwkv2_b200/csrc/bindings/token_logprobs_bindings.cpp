@@ -2,7 +2,6 @@
 // strided logits, output tensors; raw pointers and torch's current stream go to the C ABI.  No arithmetic here.
 #include "bindings.h"
 
-#include <cmath>
 #include <limits>
 #include <vector>
 
@@ -45,8 +44,7 @@ RowsShape check_logits(const torch::Tensor& logits, const torch::Tensor& token_i
   need_value(token_ids.sizes() == logits.sizes().slice(0, logits.dim() - 1),
              "token_ids must have the shape of logits without the vocabulary");
   const float t = static_cast<float>(temperature);
-  need_value(t > 0.f && std::isfinite(t) && std::isfinite(1.0f / t),
-             "temperature must be positive and finite, with a finite reciprocal in float32");
+  need_value(t >= FRWKV_TEMPERATURE_MIN && t <= FRWKV_TEMPERATURE_MAX, "temperature must be in 1e-30..1e30");
   need_value(logits.size(logits.dim() - 1) <= std::numeric_limits<int>::max() &&
                  token_ids.numel() <= std::numeric_limits<int>::max(),
              "row and vocabulary counts must fit in int32");

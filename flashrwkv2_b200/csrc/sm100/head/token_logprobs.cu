@@ -226,7 +226,7 @@ template <typename io_t> struct Part {
   bool singles;
 
   __device__ __forceinline__ int tail() const { return lead + packs * Pack<io_t>::kCount; }
-  __device__ __forceinline__ int single_count() const { return singles ? lead + vocab - tail() : 0; }
+  __device__ __forceinline__ int single_count() const { return singles ? lead + (vocab - tail()) : 0; }
   __device__ __forceinline__ int single(int i) const { return i < lead ? i : tail() + i - lead; }
   __device__ __forceinline__ int pack_id(int pack) const { return lead + pack * Pack<io_t>::kCount; }
 };
@@ -575,7 +575,7 @@ token_logprobs_backward_kernel(const Rows p, int segments, const float* __restri
   const int packs = (p.vocab - lead) / kCount;
   if (segment == 0) {
     const int tail = lead + packs * kCount;
-    for (int i = tid; i < lead + p.vocab - tail; i += kThreads) {
+    for (int i = tid; i < lead + (p.vocab - tail); i += kThreads) {
       const int j = i < lead ? i : tail + i - lead;
       out[j] = from_f32<io_t>(zero ? 0.f : one(to_f32(x[j]), j));
     }
@@ -630,8 +630,9 @@ int check_rows(const char* what, const void* logits, long long outer, long long 
     return fail(FRWKV_ERR_ARGUMENT, "%s: the row count must be positive and fit in int32", what);
   if (vocab <= 0) return fail(FRWKV_ERR_ARGUMENT, "%s: vocab must be positive", what);
   if (io_dtype < FRWKV_IO_BF16 || io_dtype > FRWKV_IO_FP32) return fail(FRWKV_ERR_UNSUPPORTED, "%s: unknown dtype", what);
-  if (!(temperature > 0.f) || !(1.0f / temperature > 0.f) || !(1.0f / temperature < INFINITY))
-    return fail(FRWKV_ERR_ARGUMENT, "%s: temperature and its reciprocal must be positive and finite", what);
+  // so that its reciprocal, times log2 e and times gradients, neither overflows (0 * inf) nor is subnormal
+  if (!(temperature >= FRWKV_TEMPERATURE_MIN && temperature <= FRWKV_TEMPERATURE_MAX))
+    return fail(FRWKV_ERR_ARGUMENT, "%s: temperature must be in 1e-30..1e30", what);
   return FRWKV_OK;
 }
 

@@ -29,7 +29,8 @@ def rl_infctx_head_token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
     two (once; the top alternatives carry no gradient).
 
     ``logits`` is ``[..., V]`` bfloat16, float16 or float32 with unit stride along V and rows that at most two strides
-    describe (so ``logits[:, :-1]`` needs no copy); ``token_ids`` int64 or int32 of shape ``[...]``; ``top_k`` 0 to 32.
+    describe (so ``logits[:, :-1]`` needs no copy); ``token_ids`` int64 or int32 of shape ``[...]``; ``temperature`` 1e-30 to
+    1e30; ``top_k`` 0 to 32.
     Equal logits rank by their ids, lowest first, and NaN ranks above all.  A row whose id is ``ignore_index`` is left
     out: logprob, entropy and gradient 0, top ids -1, top logprobs -inf.  Any other id outside the vocabulary makes that
     row's logprob and gradient NaN.  Masked logits may be -inf or the type's lowest value; in a row of -inf alone every

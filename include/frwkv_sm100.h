@@ -283,12 +283,15 @@ int frwkv_sm100_gated_scan_train_backward(
  *   ids      : int64 (ids_are_int64 nonzero) or int32; an id equal to ignore_index marks a row that
  *              is left out (logprob, entropy and gradient 0, top ids -1 and top logprobs -inf, logits not read); any
  *              other id outside [0, vocab) gives logprob and gradient NaN;
+ *   temperature : FRWKV_TEMPERATURE_MIN..MAX;
  *   stats    : fp32 [rows, 2], the row's largest logit and sum exp(z - max z): saved for the backward pass;
  *   top_ids  : int64 [rows, top_k], top_logprobs : fp32 [rows, top_k]; top_k in 0..FRWKV_TOP_K_MAX and <= vocab;
  *              descending, equal logits in the order of their ids (NaN counts as the largest);
  * A row of -inf alone has logprob and top logprobs -inf, entropy 0 and gradient 0; a NaN or +inf in a row makes its
  * logprobs, entropy and gradient NaN.  dlogprobs / dentropy : fp32 or NULL (zeros);  dlogits : contiguous [rows, vocab]. */
 #define FRWKV_TOP_K_MAX 32
+#define FRWKV_TEMPERATURE_MIN 1e-30f
+#define FRWKV_TEMPERATURE_MAX 1e30f
 int frwkv_sm100_token_logprobs(
     const void* logits, long long outer, long long inner, long long stride_outer, long long stride_inner,
     const void* ids, int ids_are_int64, long long ignore_index, int vocab, int io_dtype, float temperature, int top_k,

@@ -110,6 +110,20 @@ def test_token_logprobs_refusals(changes, error, text):
         op(**args)
 
 
+@pytest.mark.parametrize("temperature", [3e-39, 1e-38, 9e-31, 1.1e30, 3e38])
+def test_temperatures_whose_reciprocal_overflows_or_is_subnormal_are_refused(temperature):
+    """1 / 3e-39 is finite in fp32 but not times log2 e: rows would come out as NaN."""
+    from flashrwkv2_b200 import _lib, rl_infctx_head_token_logprobs as op
+
+    with pytest.raises(ValueError, match="temperature"):
+        op(torch.zeros(3, 8), torch.zeros(3, dtype=torch.int64), temperature=temperature)
+    lib = _lib.load()
+    assert lib.frwkv_sm100_token_logprobs(16, 1, 1, 8, 8, 16, 1, -100, 8, 0, temperature, 0, 16, 16, 16, 0, 0, 0) != 0
+    assert "temperature" in _lib.last_error()
+    assert lib.frwkv_sm100_token_logprobs_backward(16, 1, 1, 8, 8, 16, 1, -100, 8, 0, temperature, 16, 16, 16, 16, 16, 0) != 0
+    assert "temperature" in _lib.last_error()
+
+
 def test_operators_fail_loudly_without_backend(monkeypatch):
     import flashrwkv2_b200 as pkg
 

@@ -87,6 +87,15 @@ def test_sizes(rows, vocab, dtype):
     check_gradient(logits, ids, gradient(logits, ids, 1.0, a, b), 1.0, a, b)
 
 
+@pytest.mark.parametrize("temperature", [1e-30, 1e30])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_ends_of_the_temperature_range(dtype, temperature):
+    """At 1e-30 all of the probability is on the largest logits, at 1e30 it is even."""
+    logits, ids, a, b = case(6, 2000, dtype, seed=2)
+    check(logits, ids, score(logits, ids, temperature, 5), temperature, 5)
+    check_gradient(logits, ids, gradient(logits, ids, temperature, a, b), temperature, a, b)
+
+
 @pytest.mark.parametrize("temperature", [0.3, 1.0, 2.5, 100.0])
 @pytest.mark.parametrize("top_k", [1, 5, 32])
 def test_temperature_and_top_k(temperature, top_k):
