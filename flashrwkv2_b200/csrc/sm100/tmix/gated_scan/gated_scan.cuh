@@ -303,10 +303,12 @@ template <int V> __device__ __forceinline__ void store_states_whole(float* to, c
 template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
   using L = Lanes<V>;
 
+  static __device__ __forceinline__ L exp2(const L& x) {
+    return each([](float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }, x);
+  }
   // sigmoid(raw + bias) from bias * -log2 e, with the SFU's approximations of exp2 and the reciprocal (2^-22 each)
   static __device__ __forceinline__ L sigmoid(const L& raw, const L& bias) {
-    const L e = each([](float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; },
-                     fma(raw, L::all(-kLog2e), bias));
+    const L e = exp2(fma(raw, L::all(-kLog2e), bias));
     return each([](float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; },
                 add(e, L::all(1.0f)));
   }
@@ -351,17 +353,83 @@ template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
 };
 
 // ---- affine maps h -> a h + b
+//
+// a is the product of the rho of up to 2048 tokens, and the carried state passes through one for each 16 of them.  As one fp32
+// number it would be rounded at every token, by up to 2^-25 where its distance to one may be a millionth, and with a steady
+// decay to the same side each time (16384 tokens with 1 - rho = 1.2e-5: 8e-5 rms of the values, walked token by token 1.7e-6).
+// So the maps carry a as a sum of two numbers (2.5e-7).  It begins with a lane's tokens, whose product is known well in two
+// ways: as a - 1 where that is small, and as a where that is.
 
+// The product of the rho of a lane's tokens: from logits exp(-c times the sum of their sigmoids), else multiplied out, with the
+// sum of what each token takes away.
+template <bool LOGITS, int V> struct Fade;
+
+template <int V> struct Fade<true, V> {
+  using L = Lanes<V>;
+  L gates;
+
+  static __device__ __forceinline__ Fade none() { return Fade{L::all(0.0f)}; }
+  __device__ __forceinline__ void take(const L& sigmoid, const L&) { gates = add(gates, sigmoid); }
+  __device__ __forceinline__ L product() const { return Decay<true, false, V>::exp2(mul(gates, L::all(-kRateLog2e))); }
+  __device__ __forceinline__ L fall() const { return Decay<true, false, V>::keep_gate(gates); }  // product - 1
+  __device__ __forceinline__ L choice() const { return gates; }
+  static __device__ __forceinline__ bool is_slow(float gates) { return gates <= 1.0f; }  // fall() is good
+};
+
+template <int V> struct Fade<false, V> {
+  using L = Lanes<V>;
+  L a, less;
+
+  static __device__ __forceinline__ Fade none() { return Fade{L::all(1.0f), L::all(0.0f)}; }
+  __device__ __forceinline__ void take(const L&, const L& rho) {
+    less = fma(minus(rho, L::all(1.0f)), a, less);
+    a = mul(rho, a);
+  }
+  __device__ __forceinline__ L product() const { return a; }
+  __device__ __forceinline__ L fall() const { return less; }
+  __device__ __forceinline__ L choice() const { return a; }
+  static __device__ __forceinline__ bool is_slow(float a) { return a >= 0.5f; }
+};
+
+// `low` has a's sign and is zero only with it (so an infinite state stays one, and does not become infinity less infinity):
+// what is rounded is rounded towards zero, and where nothing is left over it is a trifle.
 template <int V> struct Map {
-  Lanes<V> a, b;
+  Lanes<V> a, low, b;  // a + low, b
 
-  static __device__ __forceinline__ Map identity() { return Map{Lanes<V>::all(1.0f), Lanes<V>::all(0.0f)}; }
-  __device__ __forceinline__ Lanes<V> apply(const Lanes<V>& h) const { return fma(a, h, b); }
+  template <bool LOGITS> static __device__ __forceinline__ Map of(const Fade<LOGITS, V>& fade, const Lanes<V>& b) {
+    const Lanes<V> one = Lanes<V>::all(1.0f), fall = fade.fall(), choice = fade.choice();
+    Lanes<V> sum;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) sum.v[i] = __fadd2_rz(one.v[i], fall.v[i]);
+    const Lanes<V> rest = add(minus(fall, minus(sum, one)), Lanes<V>::all(kTrifle));
+    Map m{fade.product(), Lanes<V>::all(0.0f), b};
+    m.low = mul(m.a, Lanes<V>::all(0x1p-30f));
+    const auto choose = [](float by, float& a, float& low, float sum, float rest) {
+      const bool slow = Fade<LOGITS, V>::is_slow(by);
+      a = slow ? sum : a;
+      low = slow ? rest : low;
+    };
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) {
+      choose(choice.v[i].x, m.a.v[i].x, m.low.v[i].x, sum.v[i].x, rest.v[i].x);
+      choose(choice.v[i].y, m.a.v[i].y, m.low.v[i].y, sum.v[i].y, rest.v[i].y);
+    }
+    return m;
+  }
+  __device__ __forceinline__ Lanes<V> apply(const Lanes<V>& h) const { return fma(a, h, fma(low, h, b)); }
   // this map, then `next`
   __device__ __forceinline__ void then(const Map& next) {
-    b = fma(next.a, b, next.b);
-    a = mul(next.a, a);
+    Lanes<V> product;
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i) product.v[i] = __fmul2_rz(a.v[i], next.a.v[i]);
+    const Lanes<V> rest = fma(a, next.a, mul(product, Lanes<V>::all(-1.0f)));
+    b = next.apply(b);
+    low = fma(a, next.low, fma(low, next.a, rest));
+    a = product;
   }
+
+ private:
+  static constexpr float kTrifle = 0x1p-50f;
 };
 
 template <int V> __device__ __forceinline__ Lanes<V> shuffle_up(const Lanes<V>& x, int lanes) {

@@ -23,7 +23,8 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
   using R = Rows<io_t, ALIGN, S>;
   extern __shared__ uint2 staged[];  // x and the decays of one tile, then dy of two: [warp][R::kWords]
   __shared__ int lengths[kRanked];
-  __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
+  __shared__ Pieces<V, CLUSTER> pieces[2][kWarps];
+  __shared__ Pieces<V, true> slots[2][CLUSTER ? kMaxCluster : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(g.dx), static_cast<io_t*>(g.ddecay), g.dinitial, p.n_seq);
@@ -94,30 +95,28 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     // with time: the gates, and what a row's gradient is multiplied by for ddecay: the state before it, less its input
     // (complement), by the gate's slope
     L kept[S], states[S];
+    Fade<LOGITS, V> fade = Fade<LOGITS, V>::none();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const L value = x[i];
-      L sigmoid;
-      if constexpr (LOGITS) {
-        sigmoid = D::sigmoid(d[i], L::all(0.0f));
-        kept[i] = D::keep_gate(sigmoid);
-      } else {
-        kept[i] = d[i];
-      }
+      L sigmoid = d[i];
+      if constexpr (LOGITS) sigmoid = D::sigmoid(sigmoid, L::all(0.0f));
+      kept[i] = LOGITS ? D::keep_gate(sigmoid) : sigmoid;
+      if (i < left) fade.take(sigmoid, kept[i]);
       states[i] = COMPLEMENT ? minus(h, value) : h;
       if constexpr (LOGITS) states[i] = mul(states[i], D::slope(sigmoid, kept[i]));
       h = D::step(kept[i], h, value);
     }
     // against it: the map of c.  Rows behind the sequence's end leave c as it is.
-    Map<V> back = Map<V>::identity();
+    L back_b = L::all(0.0f);
 #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
       if (i < left) {
-        back.b = D::fade(kept[i], add(dy[i], back.b));
-        back.a = D::fade(kept[i], back.a);
+        back_b = D::fade(kept[i], add(dy[i], back_b));
       }
     }
-    const Map<V> behind = Scan<V>::join_groups(back);
+    Map<V> back = Map<V>::of(fade, back_b);
+    join_groups(back);
     if (lane >= 32 - kLanes) pieces[buffer][warp].put(back);
     __syncwarp();  // the inputs and the decays have been read: their place is free
     fetch(next, buffer ^ 1);
@@ -128,7 +127,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
       Map<V> cta = pieces[buffer][0].get();
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w].get());
-      c = join_cluster<V>(cta, slots[buffer], carry);
+      c = join_cluster(cta, slots[buffer], carry);
       for (int w = 0; w < warp; ++w) c = pieces[buffer][w].get().apply(c);
     } else {
 #pragma unroll
@@ -137,7 +136,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
         carry = pieces[buffer][w].get().apply(carry);
       }
     }
-    c = behind.apply(c);
+    c = state_before_group(back, c);
     if (next.seq != tile.seq) carry = final_grad(next);
 
     // second sweep

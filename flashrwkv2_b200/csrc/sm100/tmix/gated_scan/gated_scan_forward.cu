@@ -19,7 +19,8 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
   using R = Rows<io_t, ALIGN, S>;
   extern __shared__ uint2 staged[];  // x of two tiles, then the decays of one: [warp][R::kWords]
   __shared__ int lengths[kRanked];
-  __shared__ Pieces<V> pieces[2][kWarps], slots[2][CLUSTER ? kMaxCluster : 1];
+  __shared__ Pieces<V, CLUSTER> pieces[2][kWarps];
+  __shared__ Pieces<V, true> slots[2][CLUSTER ? kMaxCluster : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (p.status != nullptr && p.status[0] != 0) {
     fill_rows_nan<io_t>(p, static_cast<io_t*>(p.y), nullptr, p.boundary != nullptr ? p.final_state : nullptr, p.n_seq);
@@ -90,16 +91,20 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
     const typename R::Mine x = R::mine(inputs(buffer), lane / kLanes, static_cast<const io_t*>(p.x) + own_row * p.x_stride + block_channel, p.x_stride);
     const typename R::Mine d = R::mine(decays, lane / kLanes, static_cast<const io_t*>(p.decay) + own_row * p.decay_stride + block_channel, p.decay_stride);
     L kept[S];
-    Map<V> map = Map<V>::identity();
+    L behind = L::all(0.0f);
+    Fade<LOGITS, V> fade = Fade<LOGITS, V>::none();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      kept[i] = D::keep(d[i], bias);
-      map.b = D::step(kept[i], map.b, x[i]);
-      map.a = D::fade(kept[i], map.a);
+      L sigmoid = d[i];
+      if constexpr (LOGITS) sigmoid = D::sigmoid(sigmoid, bias);
+      kept[i] = LOGITS ? D::keep_gate(sigmoid) : sigmoid;
+      behind = D::step(kept[i], behind, x[i]);
+      fade.take(sigmoid, kept[i]);
     }
     __syncwarp();  // the decays have been read: their place is free
     fetch(next, buffer ^ 1);  // in flight while this tile is joined and written
-    const Map<V> before = Scan<V>::join_groups(map);
+    Map<V> map = Map<V>::of(fade, behind);
+    join_groups(map);
     if (lane >= 32 - kLanes) pieces[buffer][warp].put(map);
     __syncthreads();
 
@@ -109,7 +114,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
       Map<V> cta = pieces[buffer][0].get();
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) cta.then(pieces[buffer][w].get());
-      h = join_cluster<V>(cta, slots[buffer], carry);
+      h = join_cluster(cta, slots[buffer], carry);
       for (int w = 0; w < warp; ++w) h = pieces[buffer][w].get().apply(h);
     } else {
 #pragma unroll
@@ -118,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
         carry = pieces[buffer][w].get().apply(carry);
       }
     }
-    h = before.apply(h);
+    h = state_before_group(map, h);
     const int left = tile.len - tile.at - own;
     if (p.boundary != nullptr && left > 0) {
       float* to = p.boundary + saved_row(tile.seq, tile.begin, tile.at + own) * p.channels + channel;

@@ -118,40 +118,59 @@ struct Tile {
   int len;    // of the sequence
 };
 
-template <int V> struct Scan {
-  using L = Lanes<V>;
-
-  // Inclusive join of the maps of a warp's lane groups, in their order; returns the map before this lane's rows.
-  static __device__ __forceinline__ Map<V> join_groups(Map<V>& m) {
-    const int lane = threadIdx.x & 31;
+// Inclusive join of the maps of a warp's lane groups, in their order.
+template <int V> __device__ __forceinline__ void join_groups(Map<V>& m) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int d = kLanes; d < 32; d *= 2) {
-      Map<V> before{shuffle_up(m.a, d), shuffle_up(m.b, d)};
-      if (lane >= d) {
-        before.then(m);
-        m = before;
-      }
+  for (int d = kLanes; d < 32; d *= 2) {
+    Map<V> before{shuffle_up(m.a, d), shuffle_up(m.low, d), shuffle_up(m.b, d)};
+    if (lane >= d) {
+      before.then(m);
+      m = before;
     }
-    Map<V> before{shuffle_up(m.a, kLanes), shuffle_up(m.b, kLanes)};
-    return lane >= kLanes ? before : Map<V>::identity();
   }
-};
+}
 
-// The maps of one warp's or CTA's rows in shared memory, by lane along the channels.
-template <int V> struct Pieces {
+// The state before a lane group's rows, from that before its warp's and the joined maps.
+template <int V> __device__ __forceinline__ Lanes<V> state_before_group(const Map<V>& joined, const Lanes<V>& warp_state) {
+  const Lanes<V> behind_previous = shuffle_up(joined.apply(warp_state), kLanes);
+  return (threadIdx.x & 31) >= kLanes ? behind_previous : warp_state;
+}
+
+// The maps of one warp's or CTA's rows in shared memory, by lane along the channels.  SHORT keeps eight bits of `low`, which is
+// 2^-23 of a at most: all of it would cost a cluster's CTAs the room of the fourth on an SM.
+template <int V, bool SHORT> struct Pieces {
   Lanes<V> a[kLanes], b[kLanes];
+  std::conditional_t<SHORT, unsigned[kLanes][V / 2], Lanes<V>[kLanes]> low;
 
   __device__ __forceinline__ void put(const Map<V>& m) {
-    a[threadIdx.x % kLanes] = m.a;
-    b[threadIdx.x % kLanes] = m.b;
+    const int at = static_cast<int>(threadIdx.x) % kLanes;
+    a[at] = m.a;
+    b[at] = m.b;
+    if constexpr (SHORT) {
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) low[at][i] = pack_pair<__nv_bfloat16>(m.low.v[i]);
+    } else {
+      low[at] = m.low;
+    }
   }
-  __device__ __forceinline__ Map<V> get() const { return Map<V>{a[threadIdx.x % kLanes], b[threadIdx.x % kLanes]}; }
+  __device__ __forceinline__ Map<V> get() const {
+    const int at = static_cast<int>(threadIdx.x) % kLanes;
+    if constexpr (SHORT) {
+      Map<V> m{a[at], Lanes<V>::all(0.0f), b[at]};
+#pragma unroll
+      for (int i = 0; i < V / 2; ++i) m.low.v[i] = make_float2(__uint_as_float(low[at][i] << 16), __uint_as_float(low[at][i] & 0xffff0000u));
+      return m;
+    } else {
+      return Map<V>{a[at], low[at], b[at]};
+    }
+  }
 };
 
 // Joins the CTAs of a cluster: each writes its map into everyone's shared memory (slots[rank]), a cluster barrier, and each
 // applies the maps of the ranks before it.  Returns the state before this CTA's tile and moves `carry` behind the cluster's.
 template <int V>
-__device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Pieces<V>* slots, Lanes<V>& carry) {
+__device__ __forceinline__ Lanes<V> join_cluster(const Map<V>& cta, Pieces<V, true>* slots, Lanes<V>& carry) {
   const cg::cluster_group cluster = cg::this_cluster();
   const int ranks = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
