@@ -303,15 +303,18 @@ template <int V> __device__ __forceinline__ void store_states_whole(float* to, c
 template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
   using L = Lanes<V>;
 
+  // The SFU's exp2 and reciprocal: errors of 2^-22 and 2^-23, those of exp2f and nearly those of a division (what they flush to
+  // zero is far below what is added to it).
   static __device__ __forceinline__ L exp2(const L& x) {
     return each([](float v) { float r; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }, x);
   }
-  // sigmoid(raw + bias) from bias * -log2 e, with the SFU's approximations of exp2 and the reciprocal (2^-22 each)
-  static __device__ __forceinline__ L sigmoid(const L& raw, const L& bias) {
-    const L e = exp2(fma(raw, L::all(-kLog2e), bias));
-    return each([](float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; },
-                add(e, L::all(1.0f)));
+  static __device__ __forceinline__ L reciprocal(const L& x) {
+    return each([](float v) { float r; asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v)); return r; }, x);
   }
+  // e = exp(-(raw + bias)) from bias * -log2 e; the sigmoid is 1 / (1 + e)
+  static __device__ __forceinline__ L exponential(const L& raw, const L& bias) { return exp2(fma(raw, L::all(-kLog2e), bias)); }
+  static __device__ __forceinline__ L sigmoid_of(const L& e) { return reciprocal(add(e, L::all(1.0f))); }
+  static __device__ __forceinline__ L sigmoid(const L& raw, const L& bias) { return sigmoid_of(exponential(raw, bias)); }
   // exp(-c g) - 1, c = exp(-1/2), 0 <= g <= 1, as g times a polynomial of degree 5: the Chebyshev interpolant of
   // (exp(-c g) - 1) / g on [0, 1], whose relative error is 5e-9 (8e-8 with fp32 arithmetic)
   static __device__ __forceinline__ L keep_gate(const L& g) {
@@ -345,9 +348,10 @@ template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
     else if constexpr (LOGITS) return mul(mul(kept, L::all(-1.0f)), g);
     else return fma(kept, mul(g, L::all(-1.0f)), g);
   }
-  // d rho / d raw from g = sigmoid(raw): -c g (1 - g) rho
-  static __device__ __forceinline__ L slope(const L& g, const L& kept) {
-    const L rest = mul(minus(L::all(1.0f), g), add(kept, L::all(1.0f)));
+  // d rho / d raw from e and g = 1 / (1 + e): -c g (1 - g) rho.  1 - g is e g, which loses nothing where g is nearly one (1 - g
+  // would be 6 % off for a logit of 16); e is infinite, or so large that g was flushed to zero, only where the slope is zero.
+  static __device__ __forceinline__ L slope(const L& e, const L& g, const L& kept) {
+    const L rest = mul(mul(each([](float v) { return fminf(v, 0x1p126f); }, e), g), add(kept, L::all(1.0f)));
     return mul(mul(g, L::all(-kRate)), rest);
   }
 };

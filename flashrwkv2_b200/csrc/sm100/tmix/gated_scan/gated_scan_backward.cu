@@ -99,12 +99,15 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
 #pragma unroll
     for (int i = 0; i < S; ++i) {
       const L value = x[i];
-      L sigmoid = d[i];
-      if constexpr (LOGITS) sigmoid = D::sigmoid(sigmoid, L::all(0.0f));
+      L sigmoid = d[i], e;
+      if constexpr (LOGITS) {
+        e = D::exponential(sigmoid, L::all(0.0f));
+        sigmoid = D::sigmoid_of(e);
+      }
       kept[i] = LOGITS ? D::keep_gate(sigmoid) : sigmoid;
       if (i < left) fade.take(sigmoid, kept[i]);
       states[i] = COMPLEMENT ? minus(h, value) : h;
-      if constexpr (LOGITS) states[i] = mul(states[i], D::slope(sigmoid, kept[i]));
+      if constexpr (LOGITS) states[i] = mul(states[i], D::slope(e, sigmoid, kept[i]));
       h = D::step(kept[i], h, value);
     }
     // against it: the map of c.  Rows behind the sequence's end leave c as it is.

@@ -100,3 +100,32 @@ def test_steady_slow_channels(decay_mode, input_mode, batch, tokens, channels):
         x.detach().view(-1, channels), decay.detach().view(-1, channels), state_pool=pool, cu_seqlens=cu,
         state_indices=torch.arange(batch, dtype=torch.int32, device=DEV), decay_mode=decay_mode, input_mode=input_mode)
     check(dict(y=served.view(batch, tokens, channels), final=pool), exact, plain, 2.0 ** -19 if logits else 0.0)
+
+
+@pytest.mark.parametrize("input_mode", ["unit", "complement"])
+def test_gradient_of_saturated_gates(input_mode):
+    """Logits of -40 to 30 and beyond, one token each: the decay's gradient against float64, relative to itself.
+
+    exp(-logit) is off by 2^-22 and by its exponent's rounding, 2^-19 for |logit| <= 44, times log 2; two sigmoids, the rest of
+    five factors: 2^-23 and 2^-24 each.  2^-18 holds all, and fp32's smallest normal number what is below it."""
+    from flashrwkv2_b200 import pretrain_tmix_gated_scan_fp32io16
+
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = torch.cat([torch.arange(-40, 40.5, 0.5), torch.tensor([-math.inf, -200.0, -100.0, -88.0, 60.0, 88.0, 120.0, math.inf])])
+        n = logits.numel()
+        g = torch.Generator().manual_seed(1)
+        x, dy = (torch.randn(1, 1, n, generator=g).to(dtype).to(DEV) for _ in range(2))
+        h0, dfinal = (torch.randn(1, n, generator=g).to(DEV) for _ in range(2))
+        decay = logits.to(dtype).view(1, 1, n).to(DEV).requires_grad_()
+        y, final = pretrain_tmix_gated_scan_fp32io16(x, decay, initial_state=h0, input_mode=input_mode)
+        got, = torch.autograd.grad((y, final), decay, (dy, dfinal))
+        s, rest = torch.sigmoid(decay.detach().double()), torch.sigmoid(-decay.detach().double())
+        slope = -RATE * s * rest * torch.exp(-RATE * s)
+        # the sum and the difference in it are fp32: their roundings do not hit the slope alone
+        dg, dh = dy.double() + dfinal.double(), h0.double() - (x.double() if input_mode == "complement" else 0.0)
+        want = dg * dh * slope
+        reach = (dy.double().abs() + dfinal.double().abs()) * (h0.double().abs() + x.double().abs()) * slope.abs()
+        allowed = 2.0 ** -18 * want.abs() + 2.0 ** -23 * reach + torch.finfo(dtype).eps / 2 * want.abs() * (1 + 2.0 ** -17)
+        allowed = allowed + 2.0 ** -126 * (1 + (dg * dh).abs())
+        allowed = torch.where(decay.detach().double().abs() <= 44, allowed, allowed + 2.0 ** -15 * want.abs())
+        assert bool(((got.double() - want).abs() <= allowed).all()), ((got.double() - want).abs() / want.abs()).max()
