@@ -92,7 +92,9 @@ torch::Tensor tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const t
     need_type(decay_bias->scalar_type() == x.scalar_type(), "decay_bias must have x's dtype");
   }
   const RowsShape s = check_tokens(x, decay_logits, true);
-  need_value(s.total >= state_indices.numel(), "every sequence needs a token");
+  // (a capacity ticket may have room for more sequences than tokens: those beyond are not active)
+  need_value(s.total >= state_indices.numel() || (validated_metadata && validated_metadata->graph_mode()),
+             "every sequence needs a token");
   check_token_devices(x, decay_logits);
   need_value(state.device() == x.device() && query_start_loc.device() == x.device() &&
                  state_indices.device() == x.device() && (!decay_bias.has_value() || decay_bias->device() == x.device()),

@@ -178,7 +178,7 @@ extern "C" int frwkv_sm100_gated_scan_train_backward(
   using namespace frwkv;
   if (!x || !decay || !boundary || !dy || !dx || !ddecay)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan backward: x, decay, boundary, dy, dx and ddecay must be non-null");
-  const int bad = check_sizes("gated_scan backward", n_seq, total_tokens, channels, io_dtype, decay_mode, input_mode);
+  const int bad = check_sizes("gated_scan backward", n_seq, total_tokens, n_seq, channels, io_dtype, decay_mode, input_mode);
   if (bad != FRWKV_OK) return bad;
   if (cu_seqlens == nullptr && total_tokens % n_seq != 0)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan backward: dense rows must be a multiple of the sequence count");

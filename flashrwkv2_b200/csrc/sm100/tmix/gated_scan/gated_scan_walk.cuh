@@ -204,10 +204,11 @@ bool multiple_of(int bytes, std::initializer_list<const void*> pointers) {
   return true;
 }
 
-int check_sizes(const char* what, int n_seq, int total, int channels, int io_dtype, int decay_mode, int input_mode) {
+// `least`: the fewest tokens that there can be.
+int check_sizes(const char* what, int n_seq, int total, int least, int channels, int io_dtype, int decay_mode, int input_mode) {
   if (n_seq <= 0 || n_seq > 65535) return fail(FRWKV_ERR_ARGUMENT, "%s: sequence count must be in 1..65535, got %d", what, n_seq);
-  if (total < n_seq || channels <= 0)
-    return fail(FRWKV_ERR_ARGUMENT, "%s: every sequence needs a token and there must be a channel", what);
+  if (total < least || channels <= 0)
+    return fail(FRWKV_ERR_ARGUMENT, "%s: there must be at least %d token(s) and a channel", what, least);
   if (channels > 0x7fffff00 || total > 0x7ffff000)
     return fail(FRWKV_ERR_UNSUPPORTED, "%s: token and channel counts must leave room for a tile below 2^31", what);
   if (io_dtype < FRWKV_IO_BF16 || io_dtype > FRWKV_IO_FP32) return fail(FRWKV_ERR_UNSUPPORTED, "%s: unknown token dtype", what);
