@@ -67,10 +67,15 @@ void check_fp32(const torch::Tensor& t, at::IntArrayRef shape, const char* name,
 
 void* optional_pointer(const std::optional<torch::Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
-torch::Tensor tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const torch::Tensor& state_indices,
-                                   const torch::Tensor& state, const torch::Tensor& x, const torch::Tensor& decay_logits,
-                                   const std::optional<torch::Tensor>& decay_bias, const TicketPtr& validated_metadata,
-                                   int64_t max_seqlen, const std::string& decay_mode, const std::string& input_mode) {
+struct Serving {
+  int mode, input;
+  RowsShape rows;
+};
+
+// Everything that can be said of a serving call without its metadata's values.
+Serving check_serving(const torch::Tensor& query_start_loc, const torch::Tensor& state_indices, const torch::Tensor& state,
+                      const torch::Tensor& x, const torch::Tensor& decay_logits, const std::optional<torch::Tensor>& decay_bias,
+                      const TicketPtr& validated_metadata, const std::string& decay_mode, const std::string& input_mode) {
   const int mode = decay_code_checked(decay_mode), input = input_code(input_mode);
   need_value(query_start_loc.dim() == 1 && state_indices.dim() == 1 && state_indices.numel() > 0 &&
                  state_indices.numel() <= 65535 && query_start_loc.numel() == state_indices.numel() + 1,
@@ -99,6 +104,23 @@ torch::Tensor tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const t
   need_value(state.device() == x.device() && query_start_loc.device() == x.device() &&
                  state_indices.device() == x.device() && (!decay_bias.has_value() || decay_bias->device() == x.device()),
              "state_pool, cu_seqlens, state_indices and decay_bias must share x's device");
+  return Serving{mode, input, s};
+}
+
+// For a caller that has the metadata of a call validated before it makes it: refusals come first.
+void check_tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const torch::Tensor& state_indices,
+                                const torch::Tensor& state, const torch::Tensor& x, const torch::Tensor& decay_logits,
+                                const std::optional<torch::Tensor>& decay_bias, const TicketPtr& validated_metadata,
+                                int64_t, const std::string& decay_mode, const std::string& input_mode) {
+  check_serving(query_start_loc, state_indices, state, x, decay_logits, decay_bias, validated_metadata, decay_mode, input_mode);
+}
+
+torch::Tensor tmix_gated_scan_fp32(const torch::Tensor& query_start_loc, const torch::Tensor& state_indices,
+                                   const torch::Tensor& state, const torch::Tensor& x, const torch::Tensor& decay_logits,
+                                   const std::optional<torch::Tensor>& decay_bias, const TicketPtr& validated_metadata,
+                                   int64_t max_seqlen, const std::string& decay_mode, const std::string& input_mode) {
+  const auto [mode, input, s] = check_serving(query_start_loc, state_indices, state, x, decay_logits, decay_bias,
+                                              validated_metadata, decay_mode, input_mode);
   const c10::cuda::CUDAGuard guard(x.device());
   const auto meta = resolve_metadata(query_start_loc, state_indices, state, x, validated_metadata, max_seqlen);
   auto y = torch::empty(x.sizes(), x.options());
@@ -235,10 +257,13 @@ std::tuple<torch::Tensor, torch::Tensor> pretrain_tmix_gated_scan(const torch::T
 }  // namespace
 
 void register_tmix_gated_scan_bindings(py::module_& module) {
-  module.def("tmix_gated_scan_fp32", &tmix_gated_scan_fp32, "Gated scan over packed rows, fp32 state in place",
-             py::arg("query_start_loc"), py::arg("state_indices"), py::arg("state"), py::arg("x"),
-             py::arg("decay_logits"), py::arg("decay_bias") = py::none(), py::arg("validated_metadata") = py::none(),
-             py::arg("max_seqlen") = -1, py::arg("decay_mode") = "logits", py::arg("input_mode") = "unit");
+  const auto serving = [&](const char* name, auto function, const char* what) {
+    module.def(name, function, what, py::arg("query_start_loc"), py::arg("state_indices"), py::arg("state"), py::arg("x"),
+               py::arg("decay_logits"), py::arg("decay_bias") = py::none(), py::arg("validated_metadata") = py::none(),
+               py::arg("max_seqlen") = -1, py::arg("decay_mode") = "logits", py::arg("input_mode") = "unit");
+  };
+  serving("tmix_gated_scan_fp32", &tmix_gated_scan_fp32, "Gated scan over packed rows, fp32 state in place");
+  serving("check_tmix_gated_scan_fp32", &check_tmix_gated_scan_fp32, "The refusals of tmix_gated_scan_fp32 alone");
   module.def("pretrain_tmix_gated_scan", &pretrain_tmix_gated_scan, "Differentiable gated scan: (y, final_state)",
              py::arg("x"), py::arg("decay_logits"), py::arg("initial_state") = py::none(), py::arg("cu_seqlens") = py::none(),
              py::arg("decay_mode") = "logits", py::arg("input_mode") = "unit");

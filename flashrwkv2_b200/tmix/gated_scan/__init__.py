@@ -11,7 +11,8 @@ moving average with a data-dependent rate).  Tokens are bfloat16, float16 or flo
 * :func:`pretrain_tmix_gated_scan_fp32io16` is differentiable, over dense or packed rows, with an initial state that
   takes a gradient and a final state that gives one.
 
-Errors: ``TypeError`` for wrong types, ``ValueError`` for wrong shapes, layouts and values, before any launch.
+Errors: ``TypeError`` for wrong types, ``ValueError`` for wrong shapes, layouts and values, before any launch; invalid
+metadata raises ``RuntimeError`` where it is validated on the host, as for the WKV7 operators.
 """
 
 from __future__ import annotations
@@ -36,13 +37,17 @@ def infer_tmix_gated_scan_fp32io16_forward_varlen(
     were allocated, and invalid metadata fills y with NaN and leaves the pool untouched.  No gradients: for those there is
     the training form."""
     native = _extension()
-    if validated_metadata is None and isinstance(x, torch.Tensor) and isinstance(state_pool, torch.Tensor) and x.is_cuda:
+
+    def call(name):
+        return getattr(native, name)(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias, validated_metadata,
+                                     -1 if max_seqlen is None else max_seqlen, decay_mode, input_mode)
+
+    if validated_metadata is None:
+        call("check_tmix_gated_scan_fp32")
         validated_metadata = prepare_tmix_wkv7_recurrent_metadata(
             cu_seqlens, state_indices, total_tokens=x.shape[0], state_pool_size=state_pool.shape[0],
             max_seqlen=max_seqlen)
-    return native.tmix_gated_scan_fp32(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias,
-                                       validated_metadata, -1 if max_seqlen is None else max_seqlen, decay_mode,
-                                       input_mode)
+    return call("tmix_gated_scan_fp32")
 
 
 __all__ = ["infer_tmix_gated_scan_fp32io16_forward_varlen", "pretrain_tmix_gated_scan_fp32io16"]

@@ -50,3 +50,37 @@ def test_a_ticket_with_room_for_more_sequences_than_tokens(tokens):
             at += length
         rest = [i for i in range(sequences) if not 7 <= i < 7 + n]
         assert torch.equal(got_pool.cpu()[rest], pool[rest])
+
+
+def serving_call(**changes):
+    g = torch.Generator().manual_seed(0)
+    args = dict(x=torch.randn(5, 6, generator=g).to(DEV), decay_logits=torch.randn(5, 6, generator=g).to(DEV),
+                state_pool=torch.ones(3, 6, device=DEV), cu_seqlens=int32(0, 2, 5), state_indices=int32(2, 0))
+    args.update(changes)
+    return args
+
+
+@pytest.mark.parametrize("changes,error,text", [
+    (dict(x=lambda: torch.zeros((), device=DEV)), ValueError, "packed shape"),
+    (dict(x=lambda: torch.zeros(5, 6, dtype=torch.float64, device=DEV)), TypeError, "bfloat16, float16 or float32"),
+    (dict(decay_logits=lambda: torch.zeros(5, 6, device=DEV, dtype=torch.bfloat16)), TypeError, "x's dtype"),
+    (dict(state_pool=lambda: torch.zeros((), device=DEV)), ValueError, "state_pool must have shape"),
+    (dict(state_pool=lambda: torch.zeros(3, 6)), ValueError, "share x's device"),
+    (dict(cu_seqlens=lambda: int32(0, 2, 5).long()), TypeError, "int32"),
+    (dict(cu_seqlens=lambda: int32(0, 2, 5).cpu()), ValueError, "share x's device"),
+    (dict(cu_seqlens=lambda: int32(0, 5)), ValueError, "cu_seqlens must have shape"),
+    (dict(cu_seqlens=lambda: None), TypeError, "incompatible function arguments"),
+    # with metadata that would be refused as well: what can be said without it comes first
+    (dict(cu_seqlens=lambda: int32(0, 5, 2), decay_mode=lambda: "exp"), ValueError, "decay_mode"),
+    (dict(state_indices=lambda: int32(9, 9), decay_bias=lambda: torch.zeros(5, device=DEV)), ValueError, "decay_bias"),
+    # and metadata that is refused where it is validated
+    (dict(cu_seqlens=lambda: int32(0, 5, 2)), RuntimeError, "query_start_loc"),
+    (dict(state_indices=lambda: int32(9, 0)), RuntimeError, "state_indices"),
+])
+def test_refusals_on_the_gpu_come_before_the_metadata(changes, error, text):
+    serve, _, _ = operators()
+    args = serving_call(**{k: v() for k, v in changes.items()})
+    with pytest.raises(error, match=text):
+        serve(**args)
+    if "state_pool" not in changes:
+        assert bool((args["state_pool"] == 1).all())
