@@ -19,7 +19,6 @@ from __future__ import annotations
 
 import torch
 
-from ..wkv7 import _checks as check
 from ..wkv7 import _extension, prepare_tmix_wkv7_recurrent_metadata
 from .pretrain import pretrain_tmix_gated_scan_fp32io16
 
@@ -38,8 +37,6 @@ def infer_tmix_gated_scan_fp32io16_forward_varlen(
     were allocated, and invalid metadata fills y with NaN and leaves the pool untouched.  No gradients: for those there is
     the training form."""
     native = _extension()
-    if max_seqlen is not None:
-        check.positive_int(max_seqlen, "max_seqlen")
 
     def call(name):
         return getattr(native, name)(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias, validated_metadata,
