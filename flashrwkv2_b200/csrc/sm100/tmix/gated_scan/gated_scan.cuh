@@ -4,6 +4,8 @@
 // From logits the kernels work with rho - 1 and write rho * h as h + (rho - 1) * h: a slow channel has 1 - rho of 1e-4
 // and less, and rho rounded to fp32 would then be off by 2^-25 / (1 - rho) of the decay it stands for, at every token
 // with the same sign.  A retention that the caller gives is used as it is (1 - rho loses a small rho instead).
+// (An infinite h becomes NaN in that form, infinity less infinity.  A second way through the rows for it, taken when one shows
+// up, made the compiler spill in the first: 64 ragged sequences of 2560 bf16 channels 414 -> 461 us.)
 #pragma once
 
 #include "../../common.cuh"

@@ -6,6 +6,10 @@
 ``input_mode`` says what enters the state: "unit" (``i_t = 1``) or "complement" (``i_t = 1 - rho_t``, an exponential
 moving average with a data-dependent rate).  Tokens are bfloat16, float16 or float32; the state is float32.
 
+A retention is a number in [0, 1].  An infinity or NaN among a channel's inputs or in its state (or a state that overflows)
+leaves the channel infinite or NaN from that token to the end of its sequence; from logits it is NaN where ``rho * inf`` would
+have kept an infinity.  Earlier tokens, other channels and other sequences are as they would be without it.
+
 * :func:`infer_tmix_gated_scan_fp32io16_forward_varlen` serves packed sequences (decode steps and prompts of any length)
   in place on a state pool, with the metadata ticket of the WKV7 operators: one ticket serves both in a step.
 * :func:`pretrain_tmix_gated_scan_fp32io16` is differentiable, over dense or packed rows, with an initial state that

@@ -84,3 +84,46 @@ def test_refusals_on_the_gpu_come_before_the_metadata(changes, error, text):
         serve(**args)
     if "state_pool" not in changes:
         assert bool((args["state_pool"] == 1).all())
+
+
+@pytest.mark.parametrize("poison", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("lengths", [[20, 900, 30], [3, 10, 2]])
+@pytest.mark.parametrize("decay_mode,input_mode", [("logits", "unit"), ("logits", "complement"), ("retention", "unit")])
+def test_where_a_bad_number_reaches(decay_mode, input_mode, lengths, poison):
+    """From its token to the end of its sequence, in its channel; every other number keeps its bits, gradients among them."""
+    serve, train, _ = operators()
+    channels, total, n = 40, sum(lengths), len(lengths)
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(total, channels, generator=g)
+    decay = torch.randn(total, channels, generator=g)
+    if decay_mode == "retention":
+        decay = torch.sigmoid(decay)
+    pool, dy = torch.randn(n, channels, generator=g), torch.randn(total, channels, generator=g).to(DEV)
+    cu = torch.tensor([0] + lengths).cumsum(0)
+    first, last = int(cu[1]), int(cu[2])
+    at = first + lengths[1] // 2
+
+    def both(x, pool):
+        state = pool.to(DEV)
+        y = serve(x.to(DEV), decay.to(DEV), state_pool=state, cu_seqlens=int32(*cu.tolist()), state_indices=int32(*range(n)),
+                  decay_mode=decay_mode, input_mode=input_mode)
+        leaves = [t.to(DEV).requires_grad_() for t in (x, decay, pool)]
+        rows, final = train(*leaves[:2], initial_state=leaves[2], cu_seqlens=int32(*cu.tolist()), decay_mode=decay_mode,
+                            input_mode=input_mode)
+        grads = torch.autograd.grad((rows, final), leaves, (dy, torch.ones_like(final)))
+        return [t.detach().cpu() for t in (y, state, rows, final, *grads)]
+
+    clean = both(x, pool)
+    x, pool = x.clone(), pool.clone()
+    x[at, 7] = poison    # an input in the middle of the second sequence
+    pool[1, 9] = poison  # and its state
+    bad = both(x, pool)
+    rows_hit = torch.zeros(total, channels, dtype=torch.bool)
+    rows_hit[at:last, 7] = rows_hit[first:last, 9] = True
+    state_hit = torch.zeros(n, channels, dtype=torch.bool)
+    state_hit[1, [7, 9]] = True
+    for k, hit in ((0, rows_hit), (1, state_hit), (2, rows_hit), (3, state_hit)):
+        assert not torch.isfinite(bad[k][hit]).any() and torch.equal(bad[k][~hit], clean[k][~hit]), k
+    # x enters no gradient but the decay's, there from its own token on (complement) or from the next
+    assert torch.equal(bad[4], clean[4]) and torch.equal(bad[6], clean[6])
+    assert torch.equal(bad[5][~rows_hit], clean[5][~rows_hit])
