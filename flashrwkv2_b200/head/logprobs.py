@@ -36,6 +36,11 @@ def rl_infctx_head_token_logprobs(logits: torch.Tensor, token_ids: torch.Tensor,
     row's logprob and gradient NaN.  Masked logits may be -inf or the type's lowest value; in a row of -inf alone every
     logprob is -inf, entropy and gradient are 0.  A NaN or +inf makes its row's results NaN.
 
+    The same call twice gives the same bits, and no row's values touch another's.  But few rows are divided among several CTAs,
+    which add up in another order: a row's float results may differ in their last bits between batches of other sizes (above and
+    below 128 and 256 rows, for wide vocabularies) and between rows at other alignments (odd vocabularies).  A policy ratio
+    between differently batched passes is 1 up to that.
+
     Errors: ``TypeError`` for wrong types, ``ValueError`` for wrong shapes, layouts and values, before any launch."""
     return TokenLogprobs(*_extension().head_token_logprobs(logits, token_ids, temperature, top_k, ignore_index))
 

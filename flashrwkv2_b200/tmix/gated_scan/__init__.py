@@ -10,6 +10,9 @@ A retention is a number in [0, 1].  An infinity or NaN among a channel's inputs 
 leaves the channel infinite or NaN from that token to the end of its sequence; from logits it is NaN where ``rho * inf`` would
 have kept an infinity.  Earlier tokens, other channels and other sequences are as they would be without it.
 
+The same call twice gives the same bits.  Which kernel and how many CTAs share a sequence follows from the shape of the whole
+batch, so a sequence's results may differ in their last bits between batches.
+
 * :func:`infer_tmix_gated_scan_fp32io16_forward_varlen` serves packed sequences (decode steps and prompts of any length)
   in place on a state pool, with the metadata ticket of the WKV7 operators: one ticket serves both in a step.
 * :func:`pretrain_tmix_gated_scan_fp32io16` is differentiable, over dense or packed rows, with an initial state that
