@@ -513,7 +513,12 @@ token_logprobs_kernel(const Rows p, int top_k, float* __restrict__ logprobs, flo
   // a row of -inf alone has no maximum and no sum; NaN shows in the sum
   const bool empty = all.m == -INFINITY && all.s == 0.f;
   const float log_s = empty ? 0.f : logf(all.s);
-  const auto logprob_of = [&](float x) { return empty ? -INFINITY : (x - all.m) * p.inv_temperature - log_s; };
+  const auto logprob_of = [&](float x) {
+    float z = (x - all.m) * p.inv_temperature;
+    // the type's lowest value far below the largest logit: a difference that only a temperature brings back into fp32's range
+    if (z == -INFINITY && x != -INFINITY) z = (0.5f * x - 0.5f * all.m) * p.inv_temperature * 2.0f;
+    return empty ? -INFINITY : z - log_s;
+  };
   if (tid == 0) {
     logprobs[row] = known ? logprob_of(given) : __int_as_float(0x7fffffff);
     entropy[row] = empty ? 0.f : log_s - all.w / all.s * 0.6931471805599453f;

@@ -57,3 +57,31 @@ def test_rows_among_other_rows(dtype, vocab):
         for key in off:
             a, b = (t[key][:8].cpu().double()[keep] for t in (told[0], first))
             assert bool(((a - b).abs() <= 2 * off[key][keep]).all()), (count, key)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("temperature", [4.0, 1e3, 1e30])
+def test_logits_further_apart_than_the_largest_number(dtype, temperature):
+    """The difference of two finite logits may pass fp32's range where the temperature brings it back."""
+    from flashrwkv2_b200 import rl_infctx_head_token_logprobs as op
+
+    big = torch.finfo(dtype).max
+    logits = torch.zeros(4, 700, dtype=dtype)
+    logits[0, 3], logits[0, 5] = big, -big
+    logits[1] = -big
+    logits[1, 699] = big
+    logits[2] = big
+    logits[2, :20] = -big
+    logits[3, 9] = -math.inf
+    ids = torch.tensor([5, 0, 7, 9])
+    out = op(logits.to(DEV), ids.to(DEV), temperature=temperature, top_k=32)
+    want = oracle.rows(logits, ids, temperature)
+    got = out.logprobs.cpu().double()
+    assert got[3] == -math.inf and bool(torch.isfinite(got[:3]).all())
+    assert bool(((got - want["logprobs"]).abs()[:3] <= want["logprobs_off"][:3]).all())
+    assert bool(((out.entropy.cpu().double() - want["entropy"]).abs() <= want["entropy_off"]).all())
+    top = oracle.top(logits, 32)
+    assert torch.equal(out.top_ids.cpu(), top)
+    told, off = (want[key].gather(-1, top) for key in ("logp", "top_off"))
+    finite = torch.isfinite(told)
+    assert bool(((out.top_logprobs.cpu().double() - told).abs()[finite] <= off[finite]).all())
