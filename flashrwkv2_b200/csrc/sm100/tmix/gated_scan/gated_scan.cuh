@@ -137,16 +137,17 @@ template <typename io_t, int ALIGN, int S> struct Rows {
     static constexpr int kPeriod = ALIGNED ? 1 : 16 / static_cast<int>(sizeof(io_t));
     unsigned at[kPeriod], shift[2];
 
-    __device__ __forceinline__ Lanes<V> operator[](int i) const {
+    __device__ __forceinline__ Lanes<V> operator[](int i) const { return unpack<io_t>(words(i)); }
+    __device__ __forceinline__ uint2 words(int i) const {
       if constexpr (ALIGNED) {
-        return unpack<io_t>((i & 1 ? odd : even)[i * kLanes]);
+        return (i & 1 ? odd : even)[i * kLanes];
       } else {
         unsigned w[3] = {0, 0, 0};
 #pragma unroll
         for (int k = 0; k < (sizeof(io_t) == 4 ? 2 : 3); ++k)
           asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[k]) : "r"(at[i % kPeriod] + i * kPitch + 4 * k) : "memory");
-        if constexpr (sizeof(io_t) == 4) return unpack<io_t>(make_uint2(w[0], w[1]));
-        return unpack<io_t>(make_uint2(__funnelshift_r(w[0], w[1], shift[i & 1]), __funnelshift_r(w[1], w[2], shift[i & 1])));
+        if constexpr (sizeof(io_t) == 4) return make_uint2(w[0], w[1]);
+        return make_uint2(__funnelshift_r(w[0], w[1], shift[i & 1]), __funnelshift_r(w[1], w[2], shift[i & 1]));
       }
     }
   };
@@ -353,8 +354,8 @@ template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
   // d rho / d raw from e and g = 1 / (1 + e): -c g (1 - g) rho.  1 - g is e g, which loses nothing where g is nearly one (1 - g
   // would be 6 % off for a logit of 16); e is infinite, or so large that g was flushed to zero, only where the slope is zero.
   static __device__ __forceinline__ L slope(const L& e, const L& g, const L& kept) {
-    const L rest = mul(mul(each([](float v) { return fminf(v, 0x1p126f); }, e), g), add(kept, L::all(1.0f)));
-    return mul(mul(g, L::all(-kRate)), rest);
+    const L rest = mul(each([](float v) { return fminf(v, 0x1p126f); }, e), g);
+    return mul(mul(rest, fma(kept, L::all(-kRate), L::all(-kRate))), g);
   }
 };
 
@@ -378,6 +379,7 @@ template <int V> struct Fade<true, V> {
   __device__ __forceinline__ void take(const L& sigmoid, const L&) { gates = add(gates, sigmoid); }
   __device__ __forceinline__ L product() const { return Decay<true, false, V>::exp2(mul(gates, L::all(-kRateLog2e))); }
   __device__ __forceinline__ L fall() const { return Decay<true, false, V>::keep_gate(gates); }  // product - 1
+  __device__ __forceinline__ L trifle() const { return L::all(0x1p-100f); }  // positive, and nothing beside a product of 16 rho
   __device__ __forceinline__ L choice() const { return gates; }
   static __device__ __forceinline__ bool is_slow(float gates) { return gates <= 1.0f; }  // fall() is good
 };
@@ -393,6 +395,7 @@ template <int V> struct Fade<false, V> {
   }
   __device__ __forceinline__ L product() const { return a; }
   __device__ __forceinline__ L fall() const { return less; }
+  __device__ __forceinline__ L trifle() const { return mul(a, L::all(0x1p-30f)); }
   __device__ __forceinline__ L choice() const { return a; }
   static __device__ __forceinline__ bool is_slow(float a) { return a >= 0.5f; }
 };
@@ -407,9 +410,8 @@ template <int V> struct Map {
     Lanes<V> sum;
 #pragma unroll
     for (int i = 0; i < V / 2; ++i) sum.v[i] = __fadd2_rz(one.v[i], fall.v[i]);
-    const Lanes<V> rest = add(minus(fall, minus(sum, one)), Lanes<V>::all(kTrifle));
-    Map m{fade.product(), Lanes<V>::all(0.0f), b};
-    m.low = mul(m.a, Lanes<V>::all(0x1p-30f));
+    const Lanes<V> rest = add(minus(fall, minus(sum, one)), Lanes<V>::all(0x1p-50f));
+    Map m{fade.product(), fade.trifle(), b};
     const auto choose = [](float by, float& a, float& low, float sum, float rest) {
       const bool slow = Fade<LOGITS, V>::is_slow(by);
       a = slow ? sum : a;
@@ -433,9 +435,6 @@ template <int V> struct Map {
     low = fma(a, next.low, fma(low, next.a, rest));
     a = product;
   }
-
- private:
-  static constexpr float kTrifle = 0x1p-50f;
 };
 
 template <int V> __device__ __forceinline__ Lanes<V> shuffle_up(const Lanes<V>& x, int lanes) {

@@ -114,9 +114,7 @@ gated_scan_backward_kernel(const GatedScanParams p, const GatedScanGrads g, cons
     L back_b = L::all(0.0f);
 #pragma unroll
     for (int i = S - 1; i >= 0; --i) {
-      if (i < left) {
-        back_b = D::fade(kept[i], add(dy[i], back_b));
-      }
+      if (i < left) back_b = D::fade(kept[i], add(dy[i], back_b));
     }
     Map<V> back = Map<V>::of(fade, back_b);
     join_groups(back);

@@ -12,7 +12,7 @@ namespace frwkv {
 namespace {
 
 template <typename io_t, int ALIGN, bool LOGITS, bool COMPLEMENT, bool CLUSTER>
-__global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
+__global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN, LOGITS, COMPLEMENT, sizeof(io_t))) gated_scan_forward_kernel(const GatedScanParams p, const Grid grid) {
   constexpr int V = 8 / sizeof(io_t);
   using L = Lanes<V>;
   using D = Decay<LOGITS, COMPLEMENT, V>;
@@ -91,15 +91,23 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
     const typename R::Mine x = R::mine(inputs(buffer), lane / kLanes, static_cast<const io_t*>(p.x) + own_row * p.x_stride + block_channel, p.x_stride);
     const typename R::Mine d = R::mine(decays, lane / kLanes, static_cast<const io_t*>(p.decay) + own_row * p.decay_stride + block_channel, p.decay_stride);
     L kept[S];
+    uint2 given[S];
+    const auto keep = [&](int i) { return LOGITS ? kept[i] : unpack<io_t>(given[i]); };
     L behind = L::all(0.0f);
     Fade<LOGITS, V> fade = Fade<LOGITS, V>::none();
 #pragma unroll
     for (int i = 0; i < S; ++i) {
-      L sigmoid = d[i];
-      if constexpr (LOGITS) sigmoid = D::sigmoid(sigmoid, bias);
-      kept[i] = LOGITS ? D::keep_gate(sigmoid) : sigmoid;
+      given[i] = d.words(i);
+      L gate = unpack<io_t>(given[i]);
+      if constexpr (LOGITS) gate = D::sigmoid(gate, bias);
+      kept[i] = LOGITS ? D::keep_gate(gate) : gate;
       behind = D::step(kept[i], behind, x[i]);
-      fade.take(sigmoid, kept[i]);
+      fade.take(gate, kept[i]);
+    }
+    if constexpr (!LOGITS) {
+      // until the second sweep the decays stay as they came, which is half the registers for 16-bit tokens
+#pragma unroll
+      for (int i = 0; i < S; ++i) asm volatile("" : "+r"(given[i].x), "+r"(given[i].y));
     }
     __syncwarp();  // the decays have been read: their place is free
     fetch(next, buffer ^ 1);  // in flight while this tile is joined and written
@@ -137,7 +145,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
     if (is_full(tile)) {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        h = D::step(kept[i], h, x[i]);
+        h = D::step(keep(i), h, x[i]);
         R::template store<true>(y, h, count);
         y += p.channels;
       }
@@ -145,7 +153,7 @@ __global__ void __launch_bounds__(kThreads, forward_ctas(ALIGN)) gated_scan_forw
     } else {
 #pragma unroll
       for (int i = 0; i < S; ++i) {
-        h = D::step(kept[i], h, x[i]);
+        h = D::step(keep(i), h, x[i]);
         if (i < left) R::template store<false>(y, h, count);
         if (i + 1 == left) store_states<V>(p.final_state + state_row(tile.seq), h, count);
         y += p.channels;
@@ -232,7 +240,7 @@ int run_forward(const GatedScanParams& p, int io_dtype, int decay_mode, int inpu
   with_type(io_dtype, alignment_of(p, io_dtype, {p.x, p.decay, p.y, p.boundary}), [&](auto io, auto align) {
     with_modes(decay_mode, input_mode, [&](auto logits, auto complement) {
       using io_t = decltype(io);
-      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(align()) * sm_count());
+      const Grid g = cut(p, max_seqlen, kLanes * 8 / static_cast<int>(sizeof(io_t)), forward_ctas(align(), logits(), complement(), sizeof(io_t)) * sm_count());
       constexpr int kWords = 3 * Rows<io_t, align(), S>::kWords;
       constexpr const char* kName = "gated_scan_forward_kernel";
       rc = g.cluster > 1 ? launch(gated_scan_forward_kernel<io_t, align(), logits(), complement(), true>, g, p, kWords, stream, kName)

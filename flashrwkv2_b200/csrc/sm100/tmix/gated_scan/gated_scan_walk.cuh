@@ -31,7 +31,10 @@ constexpr int S = 16;                // tokens of a lane in a tile
 constexpr int kWarps = kTile / (kGroups * S), kThreads = kWarps * 32;
 // CTAs per SM, by registers and by the staging of their rows.  Copies of 4 bytes go through L1, which the staging of a fourth
 // CTA would leave too small (16 x 1024 rows of 1003 fp32 channels: 86 us with four, 56 us with three).
-constexpr int forward_ctas(int align) { return align == 16 ? 4 : 3; }
+// The moving average by given retentions of 16 bits does not fit into the registers of four.
+constexpr int forward_ctas(int align, bool logits, bool complement, int element) {
+  return align == 16 && (logits || !complement || element == 4) ? 4 : 3;
+}
 constexpr int kBackwardCtas = 2;
 constexpr int kMaxCluster = 8;
 constexpr int kShortRows = 16;       // sequences of at most this many tokens are served by the step kernel
