@@ -114,9 +114,9 @@ template <typename io_t> __device__ __forceinline__ uint2 pack(const Lanes<8 / s
 // A warp's rows of one tensor: four lane groups of S rows of 64 bytes each.  ALIGN is what every row's 64 bytes begin at a
 // multiple of in global memory: 16, 4, or nothing in particular (0).  With 16 they are copied by 16 bytes, with 4 by 4.
 // Otherwise the five 16-byte pieces that a row's 64 bytes touch are copied, as far as they hold bytes of the row or of what
-// lies before it in the tensor, and a lane shifts its 8 bytes out of them.  (16 x 1024 rows of 1003 fp32 channels, by 4 bytes
-// and by pieces: forward 57 and 67 us, backward 150 and 106 us.  32 x 1024 rows of 1003 bf16 channels, element by element
-// and by pieces: 290 and 88 us, 589 and 146 us.)
+// lies before it in the tensor, and a lane shifts its 8 bytes out of them.  (When it was chosen, 16 x 1024 rows of 1003 fp32
+// channels, by 4 bytes and by pieces: forward 57 and 67 us, backward 150 and 106 us; 32 x 1024 rows of 1003 bf16 channels, element
+// by element and by pieces: 290 and 88 us, 589 and 146 us.)
 
 constexpr int kLanes = 8, kGroups = 32 / kLanes;  // lanes along the channels (8 bytes each), groups of them along time
 
@@ -363,8 +363,8 @@ template <bool LOGITS, bool COMPLEMENT, int V> struct Decay {
 //
 // a is the product of the rho of up to 2048 tokens, and the carried state passes through one for each 16 of them.  As one fp32
 // number it would be rounded at every token, by up to 2^-25 where its distance to one may be a millionth, and with a steady
-// decay to the same side each time (16384 tokens with 1 - rho = 1.2e-5: 8e-5 rms of the values, walked token by token 1.7e-6).
-// So the maps carry a as a sum of two numbers (2.5e-7).  It begins with a lane's tokens, whose product is known well in two
+// decay to the same side each time (16384 tokens with 1 - rho = 1.2e-5: 1.2e-4 rms of the values, walked token by token 1.5e-6).
+// So the maps carry a as a sum of two numbers (1.8e-7).  It begins with a lane's tokens, whose product is known well in two
 // ways: as a - 1 where that is small, and as a where that is.
 
 // The product of the rho of a lane's tokens: from logits exp(-c times the sum of their sigmoids), else multiplied out, with the

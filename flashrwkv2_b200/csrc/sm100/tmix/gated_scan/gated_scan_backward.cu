@@ -2,8 +2,8 @@
 //
 // Five elements of traffic a cell (x, decay, dy in, dx, ddecay out) and the saved states.  Gates, states and slopes are computed
 // in one sweep with time, the gradient is carried against it; both stay in registers (250 of them, so eight warps an SM, whose
-// sixteen independent rows a lane hide the latencies).  Measured on bf16 logits: 64 x 1024 x 2048 259 us = 0.79 of the HBM
-// copy rate, 8 x 4096 x 2048 141 us = 0.72 (512 units of work on 296 places: two rounds for 1.7).
+// sixteen independent rows a lane hide the latencies).  Measured on bf16 logits: 64 x 1024 x 2048 277 us = 0.74 of the HBM
+// copy rate, 8 x 4096 x 2048 153 us = 0.67 (512 units of work on 296 places: two rounds for 1.7).
 #include "gated_scan_walk.cuh"
 
 namespace frwkv {

@@ -1,10 +1,10 @@
 // Gated scan: in-place serving operator and training forward pass.
 //
 // Three elements of traffic a cell (x, decay, y), plus the state and, in training, a saved state every 16 rows: bound by HBM
-// as long as the gates' instructions (about 20 for a logit, its sigmoid and exponential among them) are hidden.  Measured on
-// bf16 logits: 64 x 2048 x 2560 318 us = 0.96 of the HBM copy rate (375 us when it runs for seconds and the power limit
-// takes the clock down: then the instructions bound it; given retentions hold 326 us), 8 x 4096 x 2048 78 us = 0.79 (512 units
-// of work on 148 SMs: some have four, some three), 1 x 65536 x 2048 190 us = 0.65 (clusters of eight: a step waits for the
+// as long as the gates' instructions (about 21 for a logit, its sigmoid and exponential among them) are hidden.  Measured on
+// bf16 logits: 64 x 2048 x 2560 335 us = 0.92 of the HBM copy rate (400 us when it runs for seconds and the power limit
+// takes the clock down: then the instructions bound it; given retentions 324 and 357 us), 8 x 4096 x 2048 83 us = 0.74 (512 units
+// of work on 148 SMs: some have four, some three), 1 x 65536 x 2048 206 us = 0.59 (clusters of eight: a step waits for the
 // cluster's barrier).
 #include "gated_scan_walk.cuh"
 

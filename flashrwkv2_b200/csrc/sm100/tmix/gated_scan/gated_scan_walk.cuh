@@ -10,8 +10,8 @@
 //
 // Why this split.  A tile walked by itself and chained to its neighbours through global memory (time split over the whole GPU
 // whatever the batch) was built first: a tile then waits for tiles that are in work beside it, 10 us of waiting for each 3 us
-// of work (130927 ragged rows of 2560 bf16 channels: 1.2 ms, here 0.35).  16 tokens a lane rather than 8 halves what the joins
-// cost (64 x 2048 rows of 2560 channels: 400 and 335 us), and 64 bytes of channels are two whole sectors of a row and give 64
+// of work (130927 ragged rows of 2560 bf16 channels: 1.2 ms, here 0.42).  16 tokens a lane rather than 8 halves what the joins
+// cost (64 x 2048 rows of 2560 channels, when it was chosen: 335 and 400 us), and 64 bytes of channels are two whole sectors of a row and give 64
 // units of work for each sequence of 2048 channels.
 #pragma once
 
@@ -31,7 +31,8 @@ constexpr int S = 16;                // tokens of a lane in a tile
 constexpr int kWarps = kTile / (kGroups * S), kThreads = kWarps * 32;
 // CTAs per SM, by registers and by the staging of their rows.  Copies of 4 bytes go through L1, which the staging of a fourth
 // CTA would leave too small (16 x 1024 rows of 1003 fp32 channels: 86 us with four, 56 us with three).
-// The moving average by given retentions of 16 bits does not fit into the registers of four.
+// The moving average by given retentions of 16 bits does not fit into the registers of four (64 x 2048 x 2560: it spills, 391 us;
+// with three 347 us).
 constexpr int forward_ctas(int align, bool logits, bool complement, int element) {
   return align == 16 && (logits || !complement || element == 4) ? 4 : 3;
 }
@@ -81,7 +82,7 @@ __device__ __forceinline__ int row_begin(const GatedScanParams& p, int seq) { re
 // By all threads of the CTA.  Long sequences that start last would leave the GPU to a few CTAs, so a batch of a few
 // sequences of different lengths is taken longest first.  Each warp ranks them for itself and takes its answer from a vote:
 // the compiler then knows that the warp agrees, and what follows from it costs one lane, not 32 (64 x 2048 rows of 2560
-// channels: 317 us; with the answer read from shared memory 370).
+// channels, when it was chosen: 317 us; with the answer read from shared memory 370).
 template <int V> __device__ __forceinline__ Unit unit_of(const GatedScanParams& p, const Grid& g, int unit, int n_seq, int* lengths) {
   const int lane = threadIdx.x & 31, chunk = unit / g.blocks;
   Unit u;
@@ -260,8 +261,8 @@ int alignment_of(const GatedScanParams& p, int io_dtype, std::initializer_list<c
 
 // How the work is cut.  Few sequences with few channels leave the GPU empty, so a cluster shares a sequence: the size that
 // needs the least time in rounds of CTAs (`slots` are resident at once) times steps, a cluster's step counting half as much
-// again.  (65536 rows of 2048 channels: 462 us for single CTAs, 259 for four, 207 for eight; 8 x 4096 rows, where 512 single
-// CTAs fill the GPU: 80 us, and 92, 100, 116 us for clusters of 2, 4, 8.)  Very many sequences are taken several to a
+// again.  (65536 rows of 2048 channels: 464 us for single CTAs, 370, 245, 207 for 2, 4, 8; 8 x 4096 rows, where 512 single
+// CTAs fill the GPU: 83 us, and 90, 98, 113 us for clusters of 2, 4, 8.)  Very many sequences are taken several to a
 // unit, so that the CTAs outlive their start.
 Grid cut(const GatedScanParams& p, int max_seqlen, int lanes, int slots) {
   Grid g{(p.channels + lanes - 1) / lanes, 1, 1};
