@@ -44,17 +44,15 @@ def infer_tmix_gated_scan_fp32io16_forward_varlen(
     were allocated, and invalid metadata fills y with NaN and leaves the pool untouched.  No gradients: for those there is
     the training form."""
     native = _extension()
-
-    def call(name):
-        return getattr(native, name)(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias, validated_metadata,
-                                     -1 if max_seqlen is None else max_seqlen, decay_mode, input_mode)
-
+    longest = -1 if max_seqlen is None else max_seqlen
     if validated_metadata is None:
-        call("check_tmix_gated_scan_fp32")
+        native.check_tmix_gated_scan_fp32(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias, None, longest,
+                                          decay_mode, input_mode)
         validated_metadata = prepare_tmix_wkv7_recurrent_metadata(
             cu_seqlens, state_indices, total_tokens=x.shape[0], state_pool_size=state_pool.shape[0],
             max_seqlen=max_seqlen)
-    return call("tmix_gated_scan_fp32")
+    return native.tmix_gated_scan_fp32(cu_seqlens, state_indices, state_pool, x, decay_logits, decay_bias,
+                                       validated_metadata, longest, decay_mode, input_mode)
 
 
 __all__ = ["infer_tmix_gated_scan_fp32io16_forward_varlen", "pretrain_tmix_gated_scan_fp32io16"]

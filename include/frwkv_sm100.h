@@ -249,6 +249,7 @@ int frwkv_sm100_wkv7_pretrain_backward(const void* r, const void* w, const void*
  *   y          : [total_tokens, channels], contiguous, token dtype;
  *   cu_seqlens, slots, status, max_seqlen : as in frwkv_sm100_wkv7_recurrent, with the same fail-closed rules
  *                (invalid metadata: y NaN-filled, pool untouched; rows behind the last active sequence untouched);
+ *                n_seq is a capacity where the status word says how many are active, and may exceed total_tokens then;
  * An infinity or NaN in a channel leaves it infinite or NaN (from logits NaN, also where rho * inf would have kept the
  * infinity) to the end of its sequence, and touches no earlier token, other channel or other sequence.
  * Any number of channels and any alignment of the element; channels, strides and starts that are multiples of 16 bytes
