@@ -289,8 +289,8 @@ extern "C" int frwkv_sm100_gated_scan(
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan: cu_seqlens, slots, state_pool, x, decay and y must be non-null");
   if (decay_bias != nullptr && decay_mode != FRWKV_DECAY_LOGITS)
     return fail(FRWKV_ERR_ARGUMENT, "gated_scan: decay_bias only applies to decay logits");
-  // with live counts n_seq is a capacity, which may exceed that of tokens
-  const int bad = check_sizes("gated_scan", n_seq, total_tokens, 1, channels, io_dtype, decay_mode, input_mode);
+  // where the status word has live counts n_seq is a capacity, which may exceed that of tokens
+  const int bad = check_sizes("gated_scan", n_seq, total_tokens, status != nullptr ? 1 : n_seq, channels, io_dtype, decay_mode, input_mode);
   if (bad != FRWKV_OK) return bad;
   // short sequences go through the step kernel, the others through the tiled one; where it is known that there are none of
   // one kind, its kernel is not launched.  (The step kernel counts its threads in 32 bits.)
